@@ -331,6 +331,138 @@ int mx_plan_schedule(const mx_plan* plan, mx_gpu_stats* stats, int32_t* primary,
 int mx_channel_mean_noalloc(const float* x, int64_t npix, int32_t c, int64_t pixel_stride, float* out,
                             void* stream);
 
+/* ------------------------------ operators on the caller's device tensors
+ * Layer norm and the dense product, each with its backward pass, over
+ * matrices in device memory: for training or serving the model's own layers
+ * (or any network built of them) outside a plan. The reference has only the
+ * forward forms, as plan ops; these entry points have no counterpart there.
+ *
+ * Common to all:
+ *   - a matrix is row-major with contiguous elements in a row and a stride (in
+ *     elements, at least the row's length) between rows, so a channel range of
+ *     a wider tensor is a matrix too. Rows whose address and stride are
+ *     multiples of 16 bytes are the fast case; any other alignment to the
+ *     element size works;
+ *   - elements are fp32, bf16 or fp16 (MX_DT_*); all sums and statistics are
+ *     held in fp32, and a result is rounded once, as it is stored;
+ *   - `stream` is a cudaStream_t (null: the legacy default stream); calls are
+ *     asynchronous on it, allocate nothing (but for 4 bytes of page-locked
+ *     host memory at a process's first call, which must come before any
+ *     stream capture), and run on the calling thread's current device, which
+ *     must be able to read the pointers;
+ *   - `workspace` is device memory, 16-byte aligned, of at least the bytes
+ *     that the _workspace query of the same arguments gives (its pointers
+ *     matter for their alignment and for being null; workspace and
+ *     workspace_bytes are ignored by it). It needs no initialisation, and may be
+ *     reused by the next call on the same stream;
+ *   - outputs may not overlap inputs or each other, unless a field says so;
+ *   - results are the same from call to call (no atomics in the sums);
+ *   - arguments are checked before anything is launched (MX_E_INVALID).
+ * Zero rows are allowed everywhere: outputs with rows are then empty, and
+ * parameter gradients are zero. */
+enum { MX_DT_F32 = 0, MX_DT_BF16 = 1, MX_DT_F16 = 2 };
+enum { MX_ACT_NONE = 0, MX_ACT_GELU = 1, MX_ACT_LRELU = 2, MX_ACT_SIGMOID = 3 };
+
+/* y[r] = (x[r] - mean[r]) * rstd[r] * scale + bias over rows of c elements,
+ * with rstd = 1 / sqrt(mean of the squared deviations + eps). mean and rstd
+ * (fp32 [rows]) are stored where not null; the backward pass reads them.
+ * y may be x itself (same stride). */
+typedef struct mx_layer_norm_args {
+  const void* x;     /* [rows][c] */
+  const void* scale; /* [c] of param_dtype */
+  const void* bias;  /* [c] of param_dtype */
+  void* y;           /* [rows][c] */
+  float* mean;       /* [rows] or null */
+  float* rstd;       /* [rows] or null */
+  int64_t rows, c;
+  int64_t x_stride, y_stride;
+  int32_t dtype;       /* of x and y */
+  int32_t param_dtype; /* dtype, or MX_DT_F32 */
+  float eps;
+  int32_t reserved;
+} mx_layer_norm_args;
+int mx_layer_norm(const mx_layer_norm_args* a, void* stream);
+
+/* The gradients of the above. With n = (x - mean) rstd and g = dy scale:
+ * dx = rstd (g - mean(g) - n mean(g n)), dscale = sum over rows of dy n,
+ * dbias = sum over rows of dy. dx null, or dscale and dbias both null, leaves
+ * that part out (dscale or dbias alone may be null too). dx may be dy itself
+ * (same stride). */
+typedef struct mx_layer_norm_backward_args {
+  const void* dy;    /* [rows][c] */
+  const void* x;     /* [rows][c] */
+  const void* scale; /* [c] of param_dtype */
+  const float* mean; /* [rows], as the forward pass stored them */
+  const float* rstd; /* [rows] */
+  void* dx;          /* [rows][c] or null */
+  void* dscale;      /* [c] of param_dtype, or null */
+  void* dbias;       /* [c] of param_dtype, or null */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t rows, c;
+  int64_t dy_stride, x_stride, dx_stride;
+  int32_t dtype;
+  int32_t param_dtype;
+} mx_layer_norm_backward_args;
+int mx_layer_norm_backward_workspace(const mx_layer_norm_backward_args* a, int64_t* bytes);
+int mx_layer_norm_backward(const mx_layer_norm_backward_args* a, void* stream);
+
+/* pre = x w^T + bias, y = act(pre) + residual. x is [m][k], w [n][k] (a 1x1
+ * convolution's [c_out][c_in]), y [m][n]. act is MX_ACT_*: GELU in its erf
+ * form, leaky ReLU with `slope`, the logistic sigmoid. fp32 products are
+ * 3xTF32 splits (about 21 significant bits a product, summed in fp32); an
+ * infinite fp32 operand gives NaN where it is used. Up to 8 rows run as plain
+ * fp32 sums. y may be the residual itself (same stride). */
+typedef struct mx_dense_args {
+  const void* x;
+  const void* w;
+  const void* bias;     /* [n] or null */
+  const void* residual; /* [m][n] or null */
+  void* y;
+  void* pre; /* [m][n], what the backward pass of an activation reads, or null */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t m, k, n;
+  int64_t x_stride, w_stride, residual_stride, y_stride, pre_stride;
+  int32_t dtype;
+  int32_t act;
+  float slope;
+  int32_t reserved;
+} mx_dense_args;
+int mx_dense_workspace(const mx_dense_args* a, int64_t* bytes);
+int mx_dense(const mx_dense_args* a, void* stream);
+
+/* The gradients of the above, with d = dy act'(pre): dx = d w, dw = d^T x,
+ * db = sum over rows of d; an output that is null is left out. The gradient
+ * of the residual is dy. pre is read where act is not MX_ACT_NONE. d is
+ * rounded to the operands' type for the two products (the tensor cores take
+ * no wider operand); db is summed before that rounding. */
+typedef struct mx_dense_backward_args {
+  const void* dy;  /* [m][n] */
+  const void* x;   /* [m][k]; may be null without dw */
+  const void* w;   /* [n][k]; may be null without dx */
+  const void* pre; /* [m][n], or null with MX_ACT_NONE */
+  void* dx;        /* [m][k] or null */
+  void* dw;        /* [n][k] or null */
+  void* db;        /* [n] or null */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t m, k, n;
+  int64_t dy_stride, x_stride, w_stride, pre_stride, dx_stride, dw_stride;
+  int32_t dtype;
+  int32_t act;
+  float slope;
+  int32_t reserved;
+} mx_dense_backward_args;
+int mx_dense_backward_workspace(const mx_dense_backward_args* a, int64_t* bytes);
+int mx_dense_backward(const mx_dense_backward_args* a, void* stream);
+
+/* Whether a dense kernel finished so far has given up a wait inside its
+ * pipeline (its output is then not to be used): MX_E_DEVICE, and the record is
+ * cleared, else MX_OK. Does not wait for any stream; mx_dense and
+ * mx_dense_backward refuse with the same status while a record stands. */
+int mx_dense_poll(void);
+
 /* ------------------------------------------------------ the batch runner
  * Independent images sharded round-robin over GPUs: one worker thread and
  * one executor handle (arena, weights, stream, graph) per device, and no

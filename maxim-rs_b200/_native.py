@@ -136,6 +136,14 @@ _SIGS = {
                                         ctypes.c_void_p, ctypes.c_int32]),
     "mx_channel_mean_noalloc": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int64,
                                                ctypes.c_void_p, ctypes.c_void_p]),
+    "mx_layer_norm": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "mx_layer_norm_backward_workspace": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]),
+    "mx_layer_norm_backward": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "mx_dense_workspace": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]),
+    "mx_dense": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "mx_dense_backward_workspace": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]),
+    "mx_dense_backward": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "mx_dense_poll": (ctypes.c_int, []),
     "mx_gpu_new_budget": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(mx_plan), ctypes.c_int64,
                                          ctypes.POINTER(ctypes.c_void_p)]),
     "mx_batch_new": (ctypes.c_int, [ctypes.POINTER(mx_batch_config), ctypes.POINTER(ctypes.c_int32), ctypes.c_int32,

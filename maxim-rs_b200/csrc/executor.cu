@@ -205,22 +205,6 @@ void split_tf32(const std::vector<float>& w, std::vector<float>& hi, std::vector
   }
 }
 
-// The driver's tensor-map encoder, looked up once per process (batch
-// workers build executors on several threads at once).
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static std::mutex mu;
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  std::lock_guard<std::mutex> l(mu);
-  if (!fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    MX_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
-    if (q != cudaDriverEntryPointSuccess || !p) throw Error("cuTensorMapEncodeTiled is unavailable", MX_E_CUDA);
-    fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  }
-  return fn;
-}
-
 // A tiled fp32 tensor map with 128-byte swizzle (the UMMA canonical layout).
 // dims / box innermost first; strides in bytes for dims 1..rank-1. Every box
 // row is 128 bytes (32 channels), and many views are channel ranges of wider
@@ -250,6 +234,22 @@ struct UmmaOp {
 };
 
 }  // namespace
+
+// The driver's tensor-map encoder, looked up once per process (batch
+// workers build executors on several threads at once).
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static std::mutex mu;
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  std::lock_guard<std::mutex> l(mu);
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    MX_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
+    if (q != cudaDriverEntryPointSuccess || !p) throw Error("cuTensorMapEncodeTiled is unavailable", MX_E_CUDA);
+    fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }
+  return fn;
+}
 }  // namespace mx
 
 struct mx_gpu {

@@ -1,6 +1,8 @@
 // Shared device-side helpers for the executor's kernels.
 #pragma once
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -26,6 +28,9 @@ struct View {
   int64_t c;  // channels of this buffer
   int64_t npix;
 };
+
+// The driver's tensor-map encoder, looked up once per process.
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
 inline unsigned blocks_for(int64_t n, int threads) { return unsigned((n + threads - 1) / threads); }
 
@@ -53,7 +58,8 @@ __device__ __forceinline__ float ex2_approx(float a) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
   return r;
 }
-__device__ __forceinline__ float gelu_f(float x) {
+// R(u) for 0 <= u <= 5.6.
+__device__ __forceinline__ float gelu_r(float u) {
   constexpr float kGeluR[12] = {
       0.4999999701976776f,
       -0.3989405930042267f,
@@ -67,10 +73,14 @@ __device__ __forceinline__ float gelu_f(float x) {
       -8.47700794111006e-05f,
       7.708666089456528e-06f,
       -3.155372496621567e-07f};
-  const float u = fminf(fabsf(x), 5.6f);
   float p = kGeluR[11];
 #pragma unroll
   for (int k = 10; k >= 0; --k) p = fmaf(p, u, kGeluR[k]);
+  return p;
+}
+__device__ __forceinline__ float gelu_f(float x) {
+  const float u = fminf(fabsf(x), 5.6f);
+  const float p = gelu_r(u);
   const float e = ex2_approx(__fmul_rn(__fmul_rn(x, -0.72134752f), x));  // 2^(-x^2 log2(e) / 2)
   return fmaf(-__fmul_rn(u, e), p, fmaxf(x, 0.0f));
 }

@@ -1,0 +1,582 @@
+// The dense product of a caller's matrices, forward and backward:
+//
+//   pre = x w^T + bias,  y = act(pre) + residual        x [m][k], w [n][k], y [m][n]
+//   d = dy act'(pre),  dx = d w,  dw = d^T x,  db = sum_rows d
+//
+// The three products are one tensor-core kernel over D[i][j] = sum_k A(i, k) B(j, k),
+// whose operands may each lie k-contiguous (K-major) or i- / j-contiguous
+// (MN-major): forward is K-major times K-major, dx takes w MN-major, and dw
+// takes both MN-major, so nothing is transposed in memory.
+#pragma once
+
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "gpu_common.cuh"
+#include "kernels_vec.cuh"
+#include "sm100.cuh"
+
+namespace mx {
+
+// ------------------------------------------------------------- activations
+__device__ __forceinline__ float act_value(int act, float v, float slope) {
+  switch (act) {
+    case MX_ACT_GELU: return gelu_f(v);
+    case MX_ACT_LRELU: return v >= 0.0f ? v : slope * v;
+    case MX_ACT_SIGMOID: return sigmoid_f(v);
+    default: return v;
+  }
+}
+
+// d/dx [x Phi(x)] = Phi(x) + x phi(x), with Phi(-u) = exp(-u^2 / 2) R(u) as in
+// gelu_f and phi(x) = exp(-x^2 / 2) / sqrt(2 pi): one exponential serves both.
+// x is clamped in the product x phi(x), which is 0 long before +-30 (an
+// infinite x would make it inf * 0).
+__device__ __forceinline__ float gelu_grad_f(float x) {
+  const float u = fminf(fabsf(x), 5.6f);
+  const float p = gelu_r(u);
+  const float e = ex2_approx(__fmul_rn(__fmul_rn(x, -0.72134752f), x));
+  const float t = e * p;  // Phi(-u)
+  const float phi = x < 0.0f ? t : 1.0f - t;
+  return fmaf(fminf(fmaxf(x, -30.0f), 30.0f) * e, 0.3989422804f, phi);
+}
+__device__ __forceinline__ float act_grad(int act, float v, float slope) {
+  switch (act) {
+    case MX_ACT_GELU: return gelu_grad_f(v);
+    case MX_ACT_LRELU: return v >= 0.0f ? 1.0f : slope;
+    case MX_ACT_SIGMOID: {
+      const float s = sigmoid_f(v);
+      return s * (1.0f - s);
+    }
+    default: return 1.0f;
+  }
+}
+
+// ----------------------------------------------------------- the epilogue
+// What happens to a sum before it is stored. With `part` set the product is
+// one of several partial sums over K: they are stored as they are, and
+// dense_join_kernel adds them and does the rest.
+struct DenseEpi {
+  const void* bias;      // [n] or null
+  const void* residual;  // [m][n] or null
+  void* y;
+  void* pre;  // null: not stored
+  int64_t residual_stride, y_stride, pre_stride;
+  int act;
+  float slope;
+  int vec_residual, vec_y, vec_pre;  // 16-byte aligned rows
+  float* part;                       // [splits][m][ldp] or null
+  int64_t ldp;                       // a multiple of 8
+};
+
+// Eight consecutive elements of a row, `valid` of which exist.
+template <class T>
+__device__ __forceinline__ void load8(const T* p, bool vec, int valid, float (&v)[8]) {
+  if (vec && valid >= 8) {
+#pragma unroll
+    for (int h = 0; h < 8 / kVec<T>; ++h) raw_unpack<T, kVec<T>>(raw_load<T, kVec<T>>(p + h * kVec<T>), v + h * kVec<T>);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < valid ? to_f(p[i]) : 0.0f;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, bool vec, int valid, const float (&v)[8]) {
+  if (vec && valid >= 8) {
+#pragma unroll
+    for (int h = 0; h < 8 / kVec<T>; ++h) raw_store<T, kVec<T>>(p + h * kVec<T>, raw_pack<T, kVec<T>>(v + h * kVec<T>));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < valid) p[i] = from_f<T>(v[i]);
+  }
+}
+
+// Bias, activation and residual of eight sums of one row, and their stores.
+template <class T>
+__device__ __forceinline__ void dense_finish(const DenseEpi& e, float (&v)[8], const float (&bias)[8], int64_t row,
+                                             int64_t col, int valid) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] += bias[i];
+  if (e.pre) store8(static_cast<T*>(e.pre) + row * e.pre_stride + col, e.vec_pre, valid, v);
+  if (e.act == MX_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) gelu_f2(v[i], v[i + 1]);
+  } else if (e.act != MX_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = act_value(e.act, v[i], e.slope);
+  }
+  if (e.residual) {
+    float r[8];
+    load8(static_cast<const T*>(e.residual) + row * e.residual_stride + col, e.vec_residual, valid, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += r[i];
+  }
+  store8(static_cast<T*>(e.y) + row * e.y_stride + col, e.vec_y, valid, v);
+}
+template <class T>
+__device__ __forceinline__ void load_bias(const DenseEpi& e, int64_t col, int valid, float (&b)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b[i] = e.bias && i < valid ? to_f(static_cast<const T*>(e.bias)[col + i]) : 0.0f;
+}
+
+// Sum of the partial products, in the order of the splits, and the epilogue.
+// One thread per 8 columns of a row.
+template <class T>
+__global__ void __launch_bounds__(256) dense_join_kernel(DenseEpi e, int splits, int64_t m, int64_t n) {
+  const int64_t cols8 = (n + 7) / 8;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < m * cols8; i += int64_t(gridDim.x) * 256) {
+    const int64_t row = i / cols8, col = (i % cols8) * 8;
+    const int valid = int(n - col < 8 ? n - col : 8);
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, b[8];
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      const float4* p = reinterpret_cast<const float4*>(e.part + (int64_t(s) * m + row) * e.ldp + col);
+      const float4 a = p[0], c = p[1];
+      v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
+      v[4] += c.x, v[5] += c.y, v[6] += c.z, v[7] += c.w;
+    }
+    load_bias<T>(e, col, valid, b);
+    dense_finish<T>(e, v, b, row, col, valid);
+  }
+}
+
+// ---------------------------------------------------- a few rows (decoding)
+// Up to R <= 8 rows of x. Then the weights are nearly all the bytes, each used
+// R times: a warp streams CPW weight rows at once (CPW 16-byte loads in
+// flight a lane) against the rows of x, which stay in the caches, with fp32
+// FMAs. Where there are few columns the KS warps of a group share the same
+// columns, each taking every KS-th vector of K, and meet in shared memory.
+template <class T, int R, int V, int CPW>
+__global__ void __launch_bounds__(256)
+    dense_rows_kernel(const T* x, int64_t x_stride, const T* w, int64_t w_stride, DenseEpi e, int m, int n, int k,
+                      int ks) {
+  __shared__ float red[8][R * CPW];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int part = warp % ks;
+  const int64_t col0 = (int64_t(blockIdx.x) * (8 / ks) + warp / ks) * CPW;
+  float acc[R][CPW];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < CPW; ++c) acc[r][c] = 0.0f;
+  if (col0 < n) {
+    // Columns past the last and rows past the last read an existing one; their sums are not stored.
+    const T* wp[CPW];
+#pragma unroll
+    for (int c = 0; c < CPW; ++c) wp[c] = w + (col0 + c < n ? col0 + c : int64_t(n) - 1) * w_stride;
+#pragma unroll 2
+    for (int i = (part * 32 + lane) * V; i < k; i += ks * 32 * V) {
+      Raw<T, V> wr[CPW];
+#pragma unroll
+      for (int c = 0; c < CPW; ++c) wr[c] = raw_load<T, V>(wp[c] + i);
+      float xv[R][V];
+#pragma unroll
+      for (int r = 0; r < R; ++r) raw_unpack<T, V>(raw_load<T, V>(x + int64_t(r < m ? r : m - 1) * x_stride + i), xv[r]);
+#pragma unroll
+      for (int c = 0; c < CPW; ++c) {
+        float wv[V];
+        raw_unpack<T, V>(wr[c], wv);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[r][c] = fmaf(xv[r][j], wv[j], acc[r][c]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < CPW; ++c) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) acc[r][c] += __shfl_xor_sync(0xFFFFFFFFu, acc[r][c], o);
+      if (lane == 0) red[warp][r * CPW + c] = acc[r][c];
+    }
+  __syncthreads();
+  if (part == 0 && lane < R * CPW) {
+    const int r = lane / CPW, c = lane % CPW;
+    const int64_t col = col0 + c;
+    if (r < m && col < n) {
+      float v = 0.0f;
+      for (int s = 0; s < ks; ++s) v += red[warp + s][lane];
+      if (e.bias) v += to_f(static_cast<const T*>(e.bias)[col]);
+      if (e.pre) static_cast<T*>(e.pre)[r * e.pre_stride + col] = from_f<T>(v);
+      v = act_value(e.act, v, e.slope);
+      if (e.residual) v += to_f(static_cast<const T*>(e.residual)[r * e.residual_stride + col]);
+      static_cast<T*>(e.y)[r * e.y_stride + col] = from_f<T>(v);
+    }
+  }
+}
+
+// ------------------------------------------ the pre-activation's gradient
+// d = dy act'(pre) and the partial column sums of d (over fp32 values, before
+// d is rounded to the operands' type for the two products). A block takes
+// 32 V columns of a range of rows, 8 rows at a time. With act none nothing is
+// written but the sums.
+template <class T, int V>
+__global__ void __launch_bounds__(256)
+    dense_grad_kernel(const T* dy, int64_t dy_stride, const T* pre, int64_t pre_stride, T* d, int64_t d_stride,
+                      float* part, int64_t m, int n, int act, float slope) {
+  __shared__ float sums[8][32 * V];
+  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
+  const int col = (blockIdx.x * 32 + lane) * V;
+  float a[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) a[k] = 0.0f;
+  if (col < n) {
+#pragma unroll 4
+    for (int64_t r = int64_t(blockIdx.y) * 8 + sub; r < m; r += int64_t(gridDim.y) * 8) {
+      float v[V];
+      raw_unpack<T, V>(raw_load<T, V>(dy + r * dy_stride + col), v);
+      if (act != MX_ACT_NONE) {
+        float q[V];
+        raw_unpack<T, V>(raw_load<T, V>(pre + r * pre_stride + col), q);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] *= act_grad(act, q[k], slope);
+        raw_store<T, V>(d + r * d_stride + col, raw_pack<T, V>(v));
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) a[k] += v[k];
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int k = 0; k < V; ++k) sums[sub][lane * V + k] = a[k];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * V; i += 256) {
+    const int cc = blockIdx.x * 32 * V + i;
+    if (cc >= n) continue;
+    float t = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 8; ++g) t += sums[g][i];
+    part[int64_t(blockIdx.y) * n + cc] = t;
+  }
+}
+
+// A copy of a matrix whose rows are not 16-byte aligned into one whose rows
+// are (what the tensor maps need). One thread per 16 bytes of the copy.
+template <class T>
+__global__ void __launch_bounds__(256)
+    dense_align_kernel(const T* src, int64_t src_stride, T* dst, int64_t dst_stride, int64_t rows, int64_t cols) {
+  constexpr int V = kVec<T>;
+  const int64_t vecs = dst_stride / V;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < rows * vecs; i += int64_t(gridDim.x) * 256) {
+    const int64_t r = i / vecs, c = (i % vecs) * V;
+    float v[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = c + k < cols ? to_f(src[r * src_stride + c + k]) : 0.0f;
+    raw_store<T, V>(dst + r * dst_stride + c, raw_pack<T, V>(v));
+  }
+}
+
+// ------------------------------------------------- the tensor-core product
+// Warp roles (one CTA per SM, persistent over output tiles of 128 x BN):
+//   warp 0       TMA producer: 128 bytes of K (64 or 32 elements) a stage
+//   warp 1       MMA issuer (one thread)
+//   warp 2       TMEM owner
+//   warps 4-11   epilogue: TMEM -> registers -> shared memory (transposing, so
+//                that rows leave in 64-byte or longer runs) -> bias,
+//                activation, residual -> memory; two warps per TMEM lane
+//                quarter, each with half the columns
+//   warps 12-19  fp32 only: the TF32 split (as in the executor's kernels:
+//                the fp32 tile itself is hi, read truncated to TF32; these
+//                warps write lo = x - hi beside it)
+// Two accumulator sets let the epilogue of one tile overlap the products of
+// the next. In fp32 a set is two regions: hi*hi, and the cross terms
+// hi*lo + lo*hi.
+// Every wait is bounded in time; one that runs out records a code in the
+// status word, and the kernel drains its copies and MMAs, frees its TMEM and
+// returns.
+struct DenseMm {
+  int64_t m, n;
+  int kb;          // k-blocks
+  int kb_split;    // k-blocks a split takes
+  int splits;
+  int tiles_m, tiles_n;
+  DenseEpi epi;
+  int* status;
+};
+
+enum : int { kDenseErrProducer = 0x201, kDenseErrSplit, kDenseErrMmaAcc, kDenseErrMmaStage, kDenseErrEpilogue };
+
+template <class T, int BN>
+struct DenseCfg {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int BK = 128 / int(sizeof(T));
+  static constexpr int A_BYTES = 128 * 128;
+  static constexpr int B_BYTES = BN * 128;
+  static constexpr int STAGE_BYTES = (A_BYTES + B_BYTES) * (F32 ? 2 : 1);
+  static constexpr int STAGES = (192 * 1024 / STAGE_BYTES) < 8 ? (192 * 1024 / STAGE_BYTES) : 8;
+  static constexpr int SET_COLS = F32 ? 2 * BN : BN;
+  static constexpr int TMEM_COLS = 2 * SET_COLS;
+  static constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
+  static constexpr int SPLIT_WARP0 = 12, SPLIT_WARPS = F32 ? 8 : 0;
+  static constexpr int THREADS = 32 * (SPLIT_WARP0 + SPLIT_WARPS);
+  // Per epilogue warp 32 rows x 32 floats; 16-byte chunk j of row r lies at
+  // j ^ (r & 7), so that neither the writes (a lane a row) nor the reads (four
+  // lanes a row) meet in a bank.
+  static constexpr int STAGING_BYTES = EPI_WARPS * 4096;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + STAGING_BYTES + 8 * (3 * STAGES + 5) + 16;
+  static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
+  static_assert(TMEM_COLS <= 512, "TMEM columns");
+};
+
+// Output tile t: groups of 8 tile rows, column by column, so that the CTAs at
+// work at one time share operand tiles in the L2.
+__device__ __forceinline__ void dense_tile(const DenseMm& p, int t, int& tm, int& tn) {
+  const int per = 8 * p.tiles_n, g = t / per, in = t % per;
+  const int rows = min(8, p.tiles_m - g * 8);
+  tm = g * 8 + in % rows;
+  tn = in / rows;
+}
+
+__device__ __forceinline__ float dense_residual(float v) {
+  // lo = v - trunc(v), rounded to TF32 (half a TF32 ulp added; the tensor core
+  // drops the low bits itself).
+  const float hi = __uint_as_float(__float_as_uint(v) & 0xFFFFE000u);
+  return __uint_as_float(__float_as_uint(__fsub_rn(v, hi)) + 0x1000u);
+}
+
+template <class T, bool A_MN, bool B_MN, int BN>
+__global__ void __launch_bounds__(DenseCfg<T, BN>::THREADS, 1)
+    dense_mm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, DenseMm p) {
+  using C = DenseCfg<T, BN>;
+  using namespace sm100;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* staging = reinterpret_cast<float*>(base + C::STAGES * C::STAGE_BYTES);
+  uint64_t* full = reinterpret_cast<uint64_t*>(base + C::STAGES * C::STAGE_BYTES + C::STAGING_BYTES);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* lo_ready = empty + C::STAGES;
+  uint64_t* acc_full = lo_ready + C::STAGES;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drained = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  __shared__ int abort_flag;
+  const volatile int* vabort = &abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int items = tiles * p.splits;
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&lo_ready[s], 32 * (C::F32 ? C::SPLIT_WARPS : 1));
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 32 * C::EPI_WARPS);
+    }
+    mbar_init(drained, 1);
+    fence_mbar_init();
+    tma_prefetch(&tmA);
+    tma_prefetch(&tmB);
+  }
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto fail = [&](int code) {
+    *static_cast<volatile int*>(p.status) = code;  // host memory: a plain store
+    abort_flag = 1;
+  };
+  auto kb_range = [&](int split, int& k0, int& k1) {
+    k0 = split * p.kb_split;
+    k1 = min(p.kb, k0 + p.kb_split);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (int w = blockIdx.x; w < items && !*vabort; w += gridDim.x) {
+        int tm, tn, k0, k1;
+        dense_tile(p, w % tiles, tm, tn);
+        kb_range(w / tiles, k0, k1);
+        for (int kb = k0; kb < k1; ++kb, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, vabort)) {
+            fail(kDenseErrProducer);
+            break;
+          }
+          uint8_t* a = base + s * C::STAGE_BYTES;
+          uint8_t* b = a + C::A_BYTES;
+          mbar_arrive_expect_tx(&full[s], C::A_BYTES + C::B_BYTES);
+          // K-major: one box of 128 (BN) rows x 128 bytes of K. MN-major: a box
+          // of BK rows of K x 128 bytes of M (N) for each 128 bytes of it.
+          if (A_MN) {
+#pragma unroll
+            for (int c = 0; c < 128 / C::BK; ++c)
+              tma_load_2d(a + c * C::BK * 128, &tmA, &full[s], tm * 128 + c * C::BK, kb * C::BK);
+          } else {
+            tma_load_2d(a, &tmA, &full[s], kb * C::BK, tm * 128);
+          }
+          if (B_MN) {
+#pragma unroll
+            for (int c = 0; c < BN / C::BK; ++c)
+              tma_load_2d(b + c * C::BK * 128, &tmB, &full[s], tn * BN + c * C::BK, kb * C::BK);
+          } else {
+            tma_load_2d(b, &tmB, &full[s], kb * C::BK, tn * BN);
+          }
+        }
+      }
+      if (*vabort)  // copies in flight land before the CTA may leave
+        for (uint32_t j = it < C::STAGES ? 0 : it - C::STAGES; j < it; ++j)
+          mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, nullptr);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc =
+          C::F32 ? idesc_tf32(128, BN, A_MN, B_MN)
+                 : idesc_f16(128, BN, A_MN, B_MN, std::is_same<T, __nv_bfloat16>::value ? 1 : 0);
+      // Steps of one MMA along K, in the descriptors' 16-byte units: 32 bytes
+      // of a K-major row, or 16 (8 in fp32) 128-byte rows of an MN-major tile.
+      constexpr uint32_t step_a = A_MN ? (C::F32 ? 64u : 128u) : 2u;
+      constexpr uint32_t step_b = B_MN ? (C::F32 ? 64u : 128u) : 2u;
+      auto desc = [](uint32_t addr, bool mn) {
+        if (!mn) return desc_kmajor_sw128(addr);
+        return C::F32 ? desc_mnmajor_sw128_32b(addr, C::BK * 128) : desc_mnmajor_sw128(addr, C::BK * 128);
+      };
+      uint32_t it = 0, tc = 0;
+      for (int w = blockIdx.x; w < items && !*vabort; w += gridDim.x, ++tc) {
+        int k0, k1;
+        kb_range(w / tiles, k0, k1);
+        const uint32_t acc = tc & 1;
+        if (!mbar_wait(&acc_empty[acc], ((tc >> 1) & 1) ^ 1, vabort)) {
+          fail(kDenseErrMmaAcc);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + acc * C::SET_COLS;
+        bool ok = true;
+        for (int kb = k0; kb < k1; ++kb, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait(C::F32 ? &lo_ready[s] : &full[s], (it / C::STAGES) & 1, vabort)) {
+            fail(kDenseErrMmaStage);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = smem_u32(base + s * C::STAGE_BYTES), b = a + C::A_BYTES;
+          const uint64_t da = desc(a, A_MN), db = desc(b, B_MN);
+          if constexpr (C::F32) {
+            const uint32_t alo = b + C::B_BYTES, blo = alo + C::A_BYTES;
+            const uint64_t dal = desc(alo, A_MN), dbl = desc(blo, B_MN);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t more = kb > k0 || k > 0;
+              mma_tf32(d, da + step_a * k, db + step_b * k, idesc, more);
+              mma_tf32(d + BN, da + step_a * k, dbl + step_b * k, idesc, more);
+              mma_tf32(d + BN, dal + step_a * k, db + step_b * k, idesc, 1u);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_f16(d, da + step_a * k, db + step_b * k, idesc, kb > k0 || k > 0);
+          }
+          mma_commit(&empty[s]);
+        }
+        if (!ok) break;
+        mma_commit(&acc_full[acc]);
+      }
+      if (*vabort) {
+        mma_commit(drained);
+        mbar_wait(drained, 0, nullptr);
+      }
+    }
+  } else if (warp >= C::EPI_WARP0 && warp < C::EPI_WARP0 + C::EPI_WARPS) {
+    const int ew = warp - C::EPI_WARP0, q = warp & 3, half = ew >> 2;
+    float4* st = reinterpret_cast<float4*>(staging + ew * 1024);
+    uint32_t tc = 0;
+    for (int w = blockIdx.x; w < items && !*vabort; w += gridDim.x, ++tc) {
+      int tm, tn;
+      dense_tile(p, w % tiles, tm, tn);
+      const int split = w / tiles;
+      const uint32_t acc = tc & 1;
+      // The warp decides as one: the TMEM loads below need all its lanes.
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[acc], (tc >> 1) & 1, vabort))) {
+        if (lane == 0) fail(kDenseErrEpilogue);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d = tmem + (uint32_t(q * 32) << 16) + acc * C::SET_COLS + half * (BN / 2);
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN / 2; c0 += 32) {
+        float v[32];
+        tmem_ld32(d + c0, v);
+        if constexpr (C::F32) {
+          float u[32];
+          tmem_ld32(d + BN + c0, u);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += u[i];
+        }
+        if (c0 + 32 == BN / 2) {  // the accumulators are read: the next tile may have them
+          tc_fence_before();
+          mbar_arrive(&acc_empty[acc]);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          st[lane * 8 + ((i / 4) ^ (lane & 7))] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        __syncwarp();
+        const int64_t col = int64_t(tn) * BN + half * (BN / 2) + c0 + (lane & 3) * 8;
+        const int valid = int(p.n - col < 8 ? p.n - col : 8);
+        float bias[8];
+        if (!p.epi.part) load_bias<T>(p.epi, col, valid, bias);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 8 + (lane >> 2);
+          const int64_t row = int64_t(tm) * 128 + q * 32 + r;
+          const float4 lo = st[r * 8 + ((2 * (lane & 3)) ^ (r & 7))];
+          const float4 hi = st[r * 8 + ((2 * (lane & 3) + 1) ^ (r & 7))];
+          if (row >= p.m || valid <= 0) continue;
+          if (p.epi.part) {
+            float4* o = reinterpret_cast<float4*>(p.epi.part + (int64_t(split) * p.m + row) * p.epi.ldp + col);
+            o[0] = lo, o[1] = hi;
+          } else {
+            float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            dense_finish<T>(p.epi, x, bias, row, col, valid);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  } else if (C::F32 && warp >= C::SPLIT_WARP0) {
+    const int tid = threadIdx.x - 32 * C::SPLIT_WARP0;
+    uint32_t it = 0;
+    for (int w = blockIdx.x; w < items && !*vabort; w += gridDim.x) {
+      int k0, k1;
+      kb_range(w / tiles, k0, k1);
+      bool ok = true;
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        const int s = it % C::STAGES;
+        if (!mbar_wait(&full[s], (it / C::STAGES) & 1, vabort)) {
+          fail(kDenseErrSplit);
+          ok = false;
+          break;
+        }
+        // Elementwise, so the swizzled layouts do not matter.
+        const float4* src = reinterpret_cast<const float4*>(base + s * C::STAGE_BYTES) + tid;
+        float4* dst = reinterpret_cast<float4*>(base + s * C::STAGE_BYTES + C::A_BYTES + C::B_BYTES) + tid;
+#pragma unroll 4
+        for (int i = 0; i < (C::A_BYTES + C::B_BYTES) / 16; i += 256) {
+          const float4 v = src[i];
+          dst[i] = make_float4(dense_residual(v.x), dense_residual(v.y), dense_residual(v.z), dense_residual(v.w));
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&lo_ready[s]);
+      }
+      if (!ok) break;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc(tmem, C::TMEM_COLS);
+}
+
+}  // namespace mx

@@ -1,0 +1,240 @@
+// Entry points of the operators on a caller's device tensors
+// (include/maxim_b200.h): argument checks and dispatch on the element type.
+#include "ops.h"
+
+#include <mutex>
+#include <string>
+
+#include "common.h"
+#include "gpu_common.cuh"
+
+namespace mx {
+namespace {
+
+const OpsTable& table(const char* who, int dtype) {
+  switch (dtype) {
+    case MX_DT_F32: return kOpsF32;
+    case MX_DT_BF16: return kOpsBf16;
+    case MX_DT_F16: return kOpsF16;
+  }
+  throw Error(fmt("%s: dtype %d is not one of MX_DT_F32, MX_DT_BF16, MX_DT_F16", who, dtype));
+}
+int64_t size_of(int dtype) { return dtype == MX_DT_F32 ? 4 : 2; }
+
+void check_size(const char* who, const char* what, int64_t v, int64_t lo) {
+  if (v < lo || v >= (int64_t(1) << 31))
+    throw Error(fmt("%s: %s = %lld is outside %lld .. 2^31-1", who, what, (long long)v, (long long)lo));
+}
+// A matrix argument: present, aligned to its elements, rows that do not overlap.
+void check_matrix(const char* who, const char* what, const void* p, int64_t rows, int64_t cols, int64_t stride,
+                  int dtype) {
+  if (rows == 0) return;
+  if (!p) throw Error(fmt("%s: %s is null", who, what));
+  if (reinterpret_cast<uintptr_t>(p) % size_of(dtype)) throw Error(fmt("%s: %s is not aligned to its elements", who, what));
+  if (stride < cols || stride >= (int64_t(1) << 36))
+    throw Error(fmt("%s: %s has a row stride of %lld; its rows have %lld elements", who, what, (long long)stride,
+                    (long long)cols));
+}
+void check_vector(const char* who, const char* what, const void* p, int dtype, bool optional) {
+  if (!p && !optional) throw Error(fmt("%s: %s is null", who, what));
+  if (reinterpret_cast<uintptr_t>(p) % size_of(dtype)) throw Error(fmt("%s: %s is not aligned to its elements", who, what));
+}
+void check_workspace(const char* who, const void* p, int64_t have, int64_t need) {
+  if (need == 0) return;
+  if (!p || have < need)
+    throw Error(fmt("%s: the workspace has %lld bytes, %lld are needed", who, (long long)(p ? have : 0), (long long)need));
+  if (reinterpret_cast<uintptr_t>(p) % 16) throw Error(fmt("%s: the workspace is not 16-byte aligned", who));
+}
+void check_act(const char* who, int act) {
+  if (act < MX_ACT_NONE || act > MX_ACT_SIGMOID) throw Error(fmt("%s: act %d is not one of MX_ACT_*", who, act));
+}
+void check_param_dtype(const char* who, int dtype, int param) {
+  if (param != dtype && param != MX_DT_F32)
+    throw Error(fmt("%s: param_dtype %d is neither the tensors' dtype nor MX_DT_F32", who, param));
+}
+
+// The status word of the dense kernels: one int of page-locked host memory
+// that every device can write, so the host reads it without a copy.
+int* g_status_host = nullptr;
+int* status_word() {
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  if (!g_status_host) {
+    void* p = nullptr;
+    MX_CUDA(cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
+    *static_cast<int*>(p) = 0;
+    g_status_host = static_cast<int*>(p);
+  }
+  return g_status_host;
+}
+
+OpsDevice device() {
+  constexpr int kMaxDevices = 64;
+  static std::mutex mu;
+  static int sms[kMaxDevices] = {};
+  int dev = 0;
+  MX_CUDA(cudaGetDevice(&dev));
+  OpsDevice d;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev < 0 || dev >= kMaxDevices) throw Error(fmt("device %d is beyond the %d the operators track", dev, kMaxDevices));
+    if (!sms[dev]) MX_CUDA(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev));
+    d.sms = sms[dev];
+  }
+  d.status = status_word();  // unified addressing: the host pointer serves the device too
+  return d;
+}
+
+void check_status(const char* who) {
+  const int code = *static_cast<volatile int*>(status_word());
+  if (code)
+    throw Error(fmt("%s: an earlier dense kernel gave up a wait in its pipeline (code 0x%x)", who, code), MX_E_DEVICE);
+}
+
+void check(const mx_layer_norm_args& a) {
+  const char* who = "mx_layer_norm";
+  table(who, a.dtype);
+  check_param_dtype(who, a.dtype, a.param_dtype);
+  check_size(who, "rows", a.rows, 0);
+  check_size(who, "c", a.c, 1);
+  check_matrix(who, "x", a.x, a.rows, a.c, a.x_stride, a.dtype);
+  check_matrix(who, "y", a.y, a.rows, a.c, a.y_stride, a.dtype);
+  check_vector(who, "scale", a.scale, a.param_dtype, false);
+  check_vector(who, "bias", a.bias, a.param_dtype, false);
+  check_vector(who, "mean", a.mean, MX_DT_F32, true);
+  check_vector(who, "rstd", a.rstd, MX_DT_F32, true);
+  if (!(a.eps >= 0.0f)) throw Error(fmt("%s: eps = %g is negative", who, double(a.eps)));
+}
+void check(const mx_layer_norm_backward_args& a) {
+  const char* who = "mx_layer_norm_backward";
+  table(who, a.dtype);
+  check_param_dtype(who, a.dtype, a.param_dtype);
+  check_size(who, "rows", a.rows, 0);
+  check_size(who, "c", a.c, 1);
+  check_matrix(who, "dy", a.dy, a.rows, a.c, a.dy_stride, a.dtype);
+  check_matrix(who, "x", a.x, a.rows, a.c, a.x_stride, a.dtype);
+  if (a.dx) check_matrix(who, "dx", a.dx, a.rows, a.c, a.dx_stride, a.dtype);
+  check_vector(who, "scale", a.scale, a.param_dtype, a.dx == nullptr);
+  check_vector(who, "mean", a.mean, MX_DT_F32, a.rows == 0);
+  check_vector(who, "rstd", a.rstd, MX_DT_F32, a.rows == 0);
+  check_vector(who, "dscale", a.dscale, a.param_dtype, true);
+  check_vector(who, "dbias", a.dbias, a.param_dtype, true);
+}
+void check(const mx_dense_args& a) {
+  const char* who = "mx_dense";
+  table(who, a.dtype);
+  check_act(who, a.act);
+  check_size(who, "m", a.m, 0);
+  check_size(who, "k", a.k, 1);
+  check_size(who, "n", a.n, 1);
+  check_matrix(who, "x", a.x, a.m, a.k, a.x_stride, a.dtype);
+  check_matrix(who, "w", a.w, a.n, a.k, a.w_stride, a.dtype);
+  check_matrix(who, "y", a.y, a.m, a.n, a.y_stride, a.dtype);
+  if (a.residual) check_matrix(who, "residual", a.residual, a.m, a.n, a.residual_stride, a.dtype);
+  if (a.pre) check_matrix(who, "pre", a.pre, a.m, a.n, a.pre_stride, a.dtype);
+  check_vector(who, "bias", a.bias, a.dtype, true);
+}
+void check(const mx_dense_backward_args& a) {
+  const char* who = "mx_dense_backward";
+  table(who, a.dtype);
+  check_act(who, a.act);
+  check_size(who, "m", a.m, 0);
+  check_size(who, "k", a.k, 1);
+  check_size(who, "n", a.n, 1);
+  check_matrix(who, "dy", a.dy, a.m, a.n, a.dy_stride, a.dtype);
+  if (a.act != MX_ACT_NONE) check_matrix(who, "pre", a.pre, a.m, a.n, a.pre_stride, a.dtype);
+  if (a.dx) {
+    check_matrix(who, "w", a.w, a.n, a.k, a.w_stride, a.dtype);
+    check_matrix(who, "dx", a.dx, a.m, a.k, a.dx_stride, a.dtype);
+  }
+  if (a.dw) {
+    check_matrix(who, "x", a.x, a.m, a.k, a.x_stride, a.dtype);
+    check_matrix(who, "dw", a.dw, a.n, a.k, a.dw_stride, a.dtype);
+  }
+  check_vector(who, "db", a.db, a.dtype, true);
+}
+
+}  // namespace
+}  // namespace mx
+
+using namespace mx;
+
+extern "C" int mx_layer_norm(const mx_layer_norm_args* a, void* stream) {
+  return guard([&] {
+    if (!a) throw Error("mx_layer_norm: null arguments");
+    check(*a);
+    if (a->rows == 0) return;
+    table("mx_layer_norm", a->dtype).layer_norm(*a, device(), static_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" int mx_layer_norm_backward_workspace(const mx_layer_norm_backward_args* a, int64_t* bytes) {
+  return guard([&] {
+    if (!a || !bytes) throw Error("mx_layer_norm_backward_workspace: null arguments");
+    check(*a);
+    *bytes = table("mx_layer_norm_backward", a->dtype).layer_norm_backward_workspace(*a, device());
+  });
+}
+
+extern "C" int mx_layer_norm_backward(const mx_layer_norm_backward_args* a, void* stream) {
+  return guard([&] {
+    if (!a) throw Error("mx_layer_norm_backward: null arguments");
+    check(*a);
+    const OpsDevice d = device();
+    const OpsTable& t = table("mx_layer_norm_backward", a->dtype);
+    check_workspace("mx_layer_norm_backward", a->workspace, a->workspace_bytes, t.layer_norm_backward_workspace(*a, d));
+    t.layer_norm_backward(*a, d, static_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" int mx_dense_workspace(const mx_dense_args* a, int64_t* bytes) {
+  return guard([&] {
+    if (!a || !bytes) throw Error("mx_dense_workspace: null arguments");
+    check(*a);
+    *bytes = table("mx_dense", a->dtype).dense_workspace(*a, device());
+  });
+}
+
+extern "C" int mx_dense(const mx_dense_args* a, void* stream) {
+  return guard([&] {
+    if (!a) throw Error("mx_dense: null arguments");
+    check(*a);
+    if (a->m == 0) return;
+    const OpsDevice d = device();
+    check_status("mx_dense");
+    const OpsTable& t = table("mx_dense", a->dtype);
+    check_workspace("mx_dense", a->workspace, a->workspace_bytes, t.dense_workspace(*a, d));
+    t.dense(*a, d, static_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" int mx_dense_backward_workspace(const mx_dense_backward_args* a, int64_t* bytes) {
+  return guard([&] {
+    if (!a || !bytes) throw Error("mx_dense_backward_workspace: null arguments");
+    check(*a);
+    *bytes = table("mx_dense_backward", a->dtype).dense_backward_workspace(*a, device());
+  });
+}
+
+extern "C" int mx_dense_backward(const mx_dense_backward_args* a, void* stream) {
+  return guard([&] {
+    if (!a) throw Error("mx_dense_backward: null arguments");
+    check(*a);
+    const OpsDevice d = device();
+    check_status("mx_dense_backward");
+    const OpsTable& t = table("mx_dense_backward", a->dtype);
+    check_workspace("mx_dense_backward", a->workspace, a->workspace_bytes, t.dense_backward_workspace(*a, d));
+    t.dense_backward(*a, d, static_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" int mx_dense_poll(void) {
+  return guard([&] {
+    volatile int* w = status_word();
+    const int code = *w;
+    if (code) {
+      *w = 0;
+      throw Error(fmt("mx_dense_poll: a dense kernel gave up a wait in its pipeline (code 0x%x)", code), MX_E_DEVICE);
+    }
+  });
+}

@@ -1,0 +1,474 @@
+// Launches of the operators on a caller's device tensors, for one element type.
+#pragma once
+
+#include <algorithm>
+#include <mutex>
+#include <string>
+
+#include "common.h"
+#include "gpu_common.cuh"
+#include "kernels_dense.cuh"
+#include "kernels_norm.cuh"
+#include "ops.h"
+
+namespace mx {
+namespace {
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+template <class T>
+constexpr int kDtype = sizeof(T) == 4 ? MX_DT_F32 : (std::is_same<T, __half>::value ? MX_DT_F16 : MX_DT_BF16);
+
+// Whether every row of a matrix starts on a 16-byte boundary.
+template <class T>
+bool aligned(const void* p, int64_t stride) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % kVec<T> == 0;
+}
+
+inline void check_launch(const char* what) {
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) throw Error(std::string(what) + ": launch: " + cudaGetErrorString(e), MX_E_CUDA);
+}
+
+// ------------------------------------------------------------- layer norm
+// The lanes a row is spread over (L) and the vectors a lane holds (NV): the
+// fewest lanes that hold the row in 16 values each, up to a warp; past that
+// a warp, then a block with 16 values a thread, then 32. f(L, NV) is called
+// with the choice as integral constants; returns false for rows too long.
+template <int V, class F>
+bool with_norm_shape(int c, F&& f) {
+  constexpr int N16 = 16 / V;
+  const int64_t vecs = ceil_div(c, V);
+#define MX_SHAPE(L, NV)                                                               \
+  if (vecs <= int64_t(L) * (NV)) {                                                    \
+    f(std::integral_constant<int, L>(), std::integral_constant<int, (NV)>());         \
+    return true;                                                                      \
+  }
+  MX_SHAPE(1, 1)
+  MX_SHAPE(2, 1)
+  MX_SHAPE(4, 1)
+  MX_SHAPE(8, 1)
+  MX_SHAPE(16, 1)
+  MX_SHAPE(32, 1)
+  if constexpr (N16 >= 4) MX_SHAPE(32, 4)
+  if constexpr (N16 != 4) MX_SHAPE(32, N16)
+  MX_SHAPE(128, N16 / 2)
+  MX_SHAPE(128, N16)
+  MX_SHAPE(256, N16)
+  MX_SHAPE(512, N16)
+  if constexpr (V > 1) MX_SHAPE(512, 2 * N16)
+#undef MX_SHAPE
+  return false;
+}
+
+template <class T, int V>
+void norm_forward_v(const mx_layer_norm_args& a, const OpsDevice& d, cudaStream_t s) {
+  NormFwd p{a.x, a.scale, a.bias, a.y, a.mean, a.rstd, a.rows, a.x_stride, a.y_stride,
+            int(a.c), a.param_dtype == MX_DT_F32, a.eps};
+  const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto nv) {
+    constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
+    constexpr int THREADS = kNormThreads<L>, GROUPS = THREADS / L;
+    const int64_t blocks = std::min<int64_t>(ceil_div(a.rows, GROUPS), int64_t(d.sms) * (1536 / THREADS));
+    layer_norm_kernel<T, V, L, NV><<<unsigned(blocks), THREADS, 0, s>>>(p);
+  });
+  if (!done) layer_norm_long_kernel<T, V><<<unsigned(std::min<int64_t>(a.rows, int64_t(d.sms) * 4)), 512, 0, s>>>(p);
+  check_launch("mx_layer_norm");
+}
+
+template <class T>
+void layer_norm(const mx_layer_norm_args& a, const OpsDevice& d, cudaStream_t s) {
+  if (aligned<T>(a.x, a.x_stride) && aligned<T>(a.y, a.y_stride) && a.c % kVec<T> == 0)
+    norm_forward_v<T, kVec<T>>(a, d, s);
+  else
+    norm_forward_v<T, 1>(a, d, s);
+}
+
+template <class T>
+bool norm_backward_vec(const mx_layer_norm_backward_args& a) {
+  return aligned<T>(a.x, a.x_stride) && aligned<T>(a.dy, a.dy_stride) && (!a.dx || aligned<T>(a.dx, a.dx_stride)) &&
+         a.c % kVec<T> == 0;
+}
+// Blocks of the backward kernel, which is also how many partial rows of the
+// parameter gradients it leaves.
+template <int V>
+int64_t norm_backward_blocks(const mx_layer_norm_backward_args& a, const OpsDevice& d) {
+  int64_t blocks = 0;
+  const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto) {
+    constexpr int L = decltype(l)::value, THREADS = kNormThreads<L>;
+    blocks = std::min<int64_t>(ceil_div(a.rows, THREADS / L), int64_t(d.sms) * (1024 / THREADS));
+  });
+  if (!done) blocks = std::min<int64_t>(ceil_div(a.rows, 8), std::max<int64_t>(1, d.sms * 4 / ceil_div(a.c, 32 * V)));
+  return blocks;
+}
+
+template <class T, int V>
+void norm_backward_v(const mx_layer_norm_backward_args& a, const OpsDevice& d, cudaStream_t s) {
+  const int64_t blocks = norm_backward_blocks<V>(a, d);
+  float* part = a.dscale || a.dbias ? static_cast<float*>(a.workspace) : nullptr;
+  NormBwd p{a.dy, a.x, a.scale, a.mean, a.rstd, a.dx, part, a.rows, a.dy_stride, a.x_stride, a.dx_stride,
+            int(a.c), a.param_dtype == MX_DT_F32};
+  const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto nv) {
+    constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
+    layer_norm_backward_kernel<T, V, L, NV><<<unsigned(blocks), kNormThreads<L>, 0, s>>>(p);
+  });
+  if (!done) {
+    // The sums first: dx may overwrite dy.
+    if (part)
+      layer_norm_param_long_kernel<T, V>
+          <<<dim3(unsigned(ceil_div(a.c, 32 * V)), unsigned(blocks)), 256, 0, s>>>(p);
+    if (a.dx)
+      layer_norm_dx_long_kernel<T, V><<<unsigned(std::min<int64_t>(a.rows, int64_t(d.sms) * 4)), 512, 0, s>>>(p);
+  }
+  check_launch("mx_layer_norm_backward");
+}
+
+// Partial rows to out0 (columns below `split`) and out1.
+template <class T>
+void join_columns(const float* part, int64_t nb, int64_t cols, int64_t split, void* out0, void* out1, bool out_f32,
+                  cudaStream_t s) {
+  const unsigned grid = unsigned(ceil_div(cols, 32));
+  if (nb <= 32)
+    column_join_kernel<T, 8><<<grid, 256, 0, s>>>(part, int(nb), cols, split, out0, out1, out_f32);
+  else
+    column_join_kernel<T, 32><<<grid, 1024, 0, s>>>(part, int(nb), cols, split, out0, out1, out_f32);
+  check_launch("column sums");
+}
+
+template <class T>
+int64_t layer_norm_backward_workspace(const mx_layer_norm_backward_args& a, const OpsDevice& d) {
+  if (!a.dscale && !a.dbias) return 0;
+  const int64_t blocks = norm_backward_vec<T>(a) ? norm_backward_blocks<kVec<T>>(a, d) : norm_backward_blocks<1>(a, d);
+  return blocks * 2 * a.c * 4;
+}
+
+template <class T>
+void layer_norm_backward(const mx_layer_norm_backward_args& a, const OpsDevice& d, cudaStream_t s) {
+  const bool out_f32 = a.param_dtype == MX_DT_F32;
+  if (a.rows == 0) {
+    const size_t bytes = size_t(a.c) * (out_f32 ? 4 : sizeof(T));
+    if (a.dscale) MX_CUDA(cudaMemsetAsync(a.dscale, 0, bytes, s));
+    if (a.dbias) MX_CUDA(cudaMemsetAsync(a.dbias, 0, bytes, s));
+    return;
+  }
+  const bool vec = norm_backward_vec<T>(a);
+  if (vec)
+    norm_backward_v<T, kVec<T>>(a, d, s);
+  else
+    norm_backward_v<T, 1>(a, d, s);
+  if (a.dscale || a.dbias)
+    join_columns<T>(static_cast<const float*>(a.workspace),
+                    vec ? norm_backward_blocks<kVec<T>>(a, d) : norm_backward_blocks<1>(a, d), 2 * a.c, a.c, a.dscale,
+                    a.dbias, out_f32, s);
+}
+
+// ------------------------------------------------------------------ dense
+// An operand of the tensor-core product: a row-major matrix whose contiguous
+// axis is the contracted one (K-major) or the other (MN-major).
+struct Operand {
+  const void* p;
+  int64_t stride;  // elements between rows
+  bool mn_major;
+};
+
+struct MmPlan {
+  int bn;
+  int splits, kb, kb_split;
+  int64_t part_bytes;
+};
+
+// Tile width and number of splits of K: the cheapest by a model of the
+// kernel's time, in units of one SM's cycles. A k-block (128 bytes of K) of a
+// 128 x BN tile costs about kStep[BN] cycles, a tile's first loads and last
+// epilogue about 3000; the CTAs of the slowest SM are what counts. Split
+// sums cost their write and reading back (about 2000 bytes a cycle for the
+// whole GPU) and another launch (about 4000).
+template <class T>
+MmPlan plan_mm(int64_t m, int64_t n, int64_t k, int sms) {
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int BK = 128 / int(sizeof(T));
+  MmPlan best{};
+  double best_cost = 0;
+  const int kb = int(ceil_div(k, BK));
+  for (int bn = 64; bn <= (F32 ? 128 : 256); bn *= 2) {
+    const int64_t tiles = ceil_div(m, 128) * ceil_div(n, bn);
+    const double step = F32 ? (bn == 64 ? 1000 : 1500) : (bn == 64 ? 250 : (bn == 128 ? 330 : 560));
+    for (int want = 1; want <= kb; want = want < 8 ? want + 1 : want * 5 / 4) {
+      if (want > 1 && tiles * want > int64_t(sms) * 2) break;
+      const int per = int(ceil_div(kb, want)), splits = int(ceil_div(kb, per));
+      const int64_t waves = ceil_div(tiles * splits, sms);
+      double cost = double(waves) * (per * step + 1000) + 3000;
+      if (splits > 1) cost += 4000 + double(splits) * double(m) * double(n) * 8 / 2000;
+      if (best.bn == 0 || cost < best_cost) {
+        best_cost = cost;
+        best = {bn, splits, kb, per, splits > 1 ? int64_t(splits) * m * round_up(n, 8) * 4 : 0};
+      }
+    }
+  }
+  return best;
+}
+
+template <class T>
+CUtensorMap operand_map(const Operand& o, int64_t rows, int64_t cols, int box_rows) {
+  constexpr int BK = 128 / int(sizeof(T));
+  const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+  const cuuint64_t strides[1] = {cuuint64_t(o.stride) * sizeof(T)};
+  const cuuint32_t box[2] = {cuuint32_t(BK), cuuint32_t(box_rows)};
+  const cuuint32_t es[2] = {1, 1};
+  const CUtensorMapDataType dt = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  // The swizzle the tensor core expects of the tile: 32-bit MN-major operands
+  // have a form of their own.
+  const CUtensorMapSwizzle sw =
+      o.mn_major && sizeof(T) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B;
+  CUtensorMap m;
+  CUresult r = tensor_map_encoder()(&m, dt, 2, const_cast<void*>(o.p), dims, strides, box, es,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw Error(fmt("cuTensorMapEncodeTiled failed (%d)", int(r)), MX_E_CUDA);
+  return m;
+}
+
+template <class T, bool A_MN, bool B_MN, int BN>
+void launch_mm(const Operand& a, const Operand& b, const DenseMm& p, int64_t k, const OpsDevice& d, cudaStream_t s) {
+  using C = DenseCfg<T, BN>;
+  constexpr int kMaxDevices = 64;
+  static std::mutex mu;
+  static bool opted[kMaxDevices] = {};
+  auto* kernel = dense_mm_kernel<T, A_MN, B_MN, BN>;
+  {
+    int dev = 0;
+    MX_CUDA(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mu);
+    if (!opted[dev]) {
+      MX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
+      opted[dev] = true;
+    }
+  }
+  const CUtensorMap ta = A_MN ? operand_map<T>(a, k, p.m, C::BK) : operand_map<T>(a, p.m, k, 128);
+  const CUtensorMap tb = B_MN ? operand_map<T>(b, k, p.n, C::BK) : operand_map<T>(b, p.n, k, BN);
+  const int64_t items = int64_t(p.tiles_m) * p.tiles_n * p.splits;
+  kernel<<<unsigned(std::min<int64_t>(items, d.sms)), C::THREADS, C::SMEM_BYTES, s>>>(ta, tb, p);
+  check_launch("dense product");
+}
+
+// D = A B^T with the epilogue `epi`: the product, and the join of its splits.
+template <class T>
+void run_mm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64_t k, DenseEpi epi, const MmPlan& plan,
+            void* part, const OpsDevice& d, cudaStream_t s) {
+  DenseMm p{};
+  p.m = m, p.n = n;
+  p.kb = plan.kb, p.kb_split = plan.kb_split, p.splits = plan.splits;
+  p.tiles_m = int(ceil_div(m, 128)), p.tiles_n = int(ceil_div(n, plan.bn));
+  p.epi = epi;
+  p.status = d.status;
+  if (plan.splits > 1) p.epi.part = static_cast<float*>(part), p.epi.ldp = round_up(n, 8);
+  auto by_width = [&](auto amn, auto bmn) {
+    constexpr bool A = decltype(amn)::value, B = decltype(bmn)::value;
+    if (plan.bn == 64) return launch_mm<T, A, B, 64>(a, b, p, k, d, s);
+    if constexpr (sizeof(T) == 2)
+      if (plan.bn == 256) return launch_mm<T, A, B, 256>(a, b, p, k, d, s);
+    launch_mm<T, A, B, 128>(a, b, p, k, d, s);
+  };
+  if (a.mn_major)
+    by_width(std::true_type(), std::true_type());
+  else if (b.mn_major)
+    by_width(std::false_type(), std::true_type());
+  else
+    by_width(std::false_type(), std::false_type());
+  if (plan.splits > 1) {
+    const int64_t vecs = m * ceil_div(n, 8);
+    dense_join_kernel<T>
+        <<<unsigned(std::min<int64_t>(ceil_div(vecs, 256), int64_t(d.sms) * 8)), 256, 0, s>>>(p.epi, plan.splits, m, n);
+    check_launch("dense join");
+  }
+}
+
+// Carves the workspace into 256-byte aligned pieces; with a null base it only counts.
+struct Carver {
+  uint8_t* base;
+  int64_t used = 0;
+  void* take(int64_t bytes) {
+    if (bytes == 0) return nullptr;
+    void* p = base ? base + used : nullptr;
+    used += round_up(bytes, 256);
+    return p;
+  }
+};
+// The workspace is 16-byte aligned only; the pieces' alignment is relative to it.
+
+// A matrix the tensor maps can take: itself, or an aligned copy.
+template <class T>
+struct Staged {
+  const void* src;
+  int64_t src_stride, rows, cols;
+  T* copy;
+  int64_t stride;
+  Staged(Carver& c, const void* p, int64_t st, int64_t r, int64_t n)
+      : src(p), src_stride(st), rows(r), cols(n), copy(nullptr), stride(st) {
+    if (!aligned<T>(p, st)) {
+      stride = round_up(n, kVec<T>);
+      copy = static_cast<T*>(c.take(rows * stride * int64_t(sizeof(T))));
+    }
+  }
+  Operand ready(bool mn_major, const OpsDevice& d, cudaStream_t s) const {
+    if (!copy) return {src, stride, mn_major};
+    const int64_t vecs = rows * stride / kVec<T>;
+    dense_align_kernel<T><<<unsigned(std::min<int64_t>(ceil_div(vecs, 256), int64_t(d.sms) * 16)), 256, 0, s>>>(
+        static_cast<const T*>(src), src_stride, copy, stride, rows, cols);
+    check_launch("aligned copy");
+    return {copy, stride, mn_major};
+  }
+};
+
+constexpr int kRowsMax = 8;  // rows the FMA kernel takes
+
+template <class T>
+int64_t dense_workspace(const mx_dense_args& a, const OpsDevice& d) {
+  if (a.m <= kRowsMax) return 0;
+  Carver c{nullptr};
+  Staged<T> x(c, a.x, a.x_stride, a.m, a.k), w(c, a.w, a.w_stride, a.n, a.k);
+  c.take(plan_mm<T>(a.m, a.n, a.k, d.sms).part_bytes);
+  return c.used;
+}
+
+template <class T>
+void dense_rows(const mx_dense_args& a, const DenseEpi& epi, const OpsDevice& d, cudaStream_t s) {
+  const bool vec = aligned<T>(a.x, a.x_stride) && aligned<T>(a.w, a.w_stride) && a.k % kVec<T> == 0;
+  // Four weight rows a warp where that still gives every SM a dozen warps,
+  // else one; and then as many warps on one row as keep the SMs busy and
+  // have a vector of K each.
+  const int cpw = a.n >= int64_t(d.sms) * 48 ? 4 : 1;
+  const int64_t vecs = ceil_div(a.k, (vec ? kVec<T> : 1) * 32);
+  int ks = 1;
+  while (ks < 8 && ks < vecs && ceil_div(a.n, cpw) * ks < int64_t(d.sms) * 16) ks *= 2;
+  const unsigned grid = unsigned(ceil_div(ceil_div(a.n, cpw), 8 / ks));
+  auto go = [&](auto r, auto v, auto c) {
+    dense_rows_kernel<T, decltype(r)::value, decltype(v)::value, decltype(c)::value><<<grid, 256, 0, s>>>(
+        static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.w), a.w_stride, epi, int(a.m), int(a.n),
+        int(a.k), ks);
+  };
+  auto by_cols = [&](auto r, auto v) {
+    if (cpw == 4)
+      go(r, v, std::integral_constant<int, 4>());
+    else
+      go(r, v, std::integral_constant<int, 1>());
+  };
+  auto by_vec = [&](auto r) {
+    if (vec)
+      by_cols(r, std::integral_constant<int, kVec<T>>());
+    else
+      by_cols(r, std::integral_constant<int, 1>());
+  };
+  if (a.m == 1)
+    by_vec(std::integral_constant<int, 1>());
+  else if (a.m <= 4)
+    by_vec(std::integral_constant<int, 4>());
+  else
+    by_vec(std::integral_constant<int, 8>());
+  check_launch("mx_dense");
+}
+
+template <class T>
+void dense(const mx_dense_args& a, const OpsDevice& d, cudaStream_t s) {
+  DenseEpi e{};
+  e.bias = a.bias, e.residual = a.residual, e.y = a.y, e.pre = a.pre;
+  e.residual_stride = a.residual_stride, e.y_stride = a.y_stride, e.pre_stride = a.pre_stride;
+  e.act = a.act, e.slope = a.slope;
+  e.vec_residual = a.residual && aligned<T>(a.residual, a.residual_stride);
+  e.vec_y = aligned<T>(a.y, a.y_stride);
+  e.vec_pre = a.pre && aligned<T>(a.pre, a.pre_stride);
+  if (a.m <= kRowsMax) return dense_rows<T>(a, e, d, s);
+  Carver c{static_cast<uint8_t*>(a.workspace)};
+  Staged<T> x(c, a.x, a.x_stride, a.m, a.k), w(c, a.w, a.w_stride, a.n, a.k);
+  const MmPlan plan = plan_mm<T>(a.m, a.n, a.k, d.sms);
+  void* part = c.take(plan.part_bytes);
+  const Operand oa = x.ready(false, d, s), ob = w.ready(false, d, s);
+  run_mm<T>(oa, ob, a.m, a.n, a.k, e, plan, part, d, s);
+}
+
+// The pieces of the backward pass and where they lie in the workspace.
+template <class T>
+struct DenseBackward {
+  const bool act, products;
+  bool vec;               // 16-byte accesses to dy, pre and d
+  int64_t chunks;         // row ranges of the column sums
+  T* d;                   // dy act'(pre), rounded to T
+  int64_t d_stride;
+  float* db_part;
+  Staged<T> dy, x, w;
+  MmPlan dx, dw;
+  void* part;
+  DenseBackward(Carver& c, const mx_dense_backward_args& a, const OpsDevice& dev)
+      : act(a.act != MX_ACT_NONE), products(a.dx || a.dw), vec(false), chunks(0),
+        d(nullptr), d_stride(round_up(a.n, kVec<T>)), db_part(nullptr),
+        // Without an activation d is dy itself.
+        dy(c, act || !products ? nullptr : a.dy, act || !products ? 0 : a.dy_stride, a.m, a.n),
+        x(c, a.dw ? a.x : nullptr, a.dw ? a.x_stride : 0, a.m, a.k),
+        w(c, a.dx ? a.w : nullptr, a.dx ? a.w_stride : 0, a.n, a.k), dx{}, dw{}, part(nullptr) {
+    vec = aligned<T>(a.dy, a.dy_stride) && (!act || aligned<T>(a.pre, a.pre_stride)) && a.n % kVec<T> == 0;
+    if (act || a.db) {
+      const int64_t cols = ceil_div(a.n, 32 * (vec ? kVec<T> : 1));
+      chunks = std::min<int64_t>(ceil_div(a.m, 16), std::max<int64_t>(1, int64_t(dev.sms) * 6 / cols));
+    }
+    if (act) d = static_cast<T*>(c.take(a.m * d_stride * int64_t(sizeof(T))));
+    if (a.db) db_part = static_cast<float*>(c.take(chunks * a.n * 4));
+    if (a.dx) dx = plan_mm<T>(a.m, a.k, a.n, dev.sms);
+    if (a.dw) dw = plan_mm<T>(a.n, a.k, a.m, dev.sms);
+    part = c.take(std::max(dx.part_bytes, dw.part_bytes));  // the products run one after the other
+  }
+};
+
+template <class T>
+int64_t dense_backward_workspace(const mx_dense_backward_args& a, const OpsDevice& dev) {
+  if (a.m == 0) return 0;
+  Carver c{nullptr};
+  DenseBackward<T> b(c, a, dev);
+  return c.used;
+}
+
+template <class T>
+void dense_backward(const mx_dense_backward_args& a, const OpsDevice& dev, cudaStream_t s) {
+  if (a.m == 0) {
+    if (a.dw) MX_CUDA(cudaMemset2DAsync(a.dw, size_t(a.dw_stride) * sizeof(T), 0, size_t(a.k) * sizeof(T), a.n, s));
+    if (a.db) MX_CUDA(cudaMemsetAsync(a.db, 0, size_t(a.n) * sizeof(T), s));
+    return;
+  }
+  Carver c{static_cast<uint8_t*>(a.workspace)};
+  DenseBackward<T> b(c, a, dev);
+  if (b.act || a.db) {
+    auto go = [&](auto v) {
+      constexpr int V = decltype(v)::value;
+      dense_grad_kernel<T, V><<<dim3(unsigned(ceil_div(a.n, 32 * V)), unsigned(b.chunks)), 256, 0, s>>>(
+          static_cast<const T*>(a.dy), a.dy_stride, static_cast<const T*>(a.pre), a.pre_stride, b.d, b.d_stride,
+          b.db_part, a.m, int(a.n), a.act, a.slope);
+    };
+    if (b.vec)
+      go(std::integral_constant<int, kVec<T>>());
+    else
+      go(std::integral_constant<int, 1>());
+    check_launch("mx_dense_backward");
+    if (a.db) join_columns<T>(b.db_part, b.chunks, a.n, a.n, a.db, nullptr, false, s);
+  }
+  if (!b.products) return;
+  const Operand d = b.act ? Operand{b.d, b.d_stride, false} : b.dy.ready(false, dev, s);
+  DenseEpi e{};
+  if (a.dx) {
+    e.y = a.dx, e.y_stride = a.dx_stride, e.vec_y = aligned<T>(a.dx, a.dx_stride);
+    run_mm<T>(d, b.w.ready(true, dev, s), a.m, a.k, a.n, e, b.dx, b.part, dev, s);
+  }
+  if (a.dw) {
+    e.y = a.dw, e.y_stride = a.dw_stride, e.vec_y = aligned<T>(a.dw, a.dw_stride);
+    run_mm<T>({d.p, d.stride, true}, b.x.ready(true, dev, s), a.n, a.k, a.m, e, b.dw, b.part, dev, s);
+  }
+}
+
+template <class T>
+constexpr OpsTable ops_table() {
+  return {layer_norm<T>,      layer_norm_backward_workspace<T>, layer_norm_backward<T>, dense_workspace<T>, dense<T>,
+          dense_backward_workspace<T>, dense_backward<T>};
+}
+
+}  // namespace
+}  // namespace mx

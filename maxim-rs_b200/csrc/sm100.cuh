@@ -177,6 +177,17 @@ __device__ __forceinline__ void mma_tf32_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// D[tmem] (+)= A[smem] * B[smem]^T, one instruction of K = 16, kind::f16
+// (both operands fp16, or both bf16).
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // Store 32 consecutive 32-bit columns of this warp's 32 lanes (thread t
 // writes row lane base + t); tmem_wait_st waits until they have landed.
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
@@ -298,10 +309,30 @@ __device__ __forceinline__ uint64_t desc_mnmajor_sw128_32b(uint32_t addr, uint32
   d |= uint64_t(1) << 61;  // SWIZZLE_128B_BASE32B
   return d;
 }
+// A 16-bit MN-major operand in the 128-byte-swizzled layout: 128-byte rows of
+// 64 elements along MN, one row per K index, 8 K-rows per 1024-byte atom.
+// `lbo` is the byte distance between consecutive 64-wide MN chunks.
+__device__ __forceinline__ uint64_t desc_mnmajor_sw128(uint32_t addr, uint32_t lbo) {
+  uint64_t d = 0;
+  d |= uint64_t((addr >> 4) & 0x3FFF);
+  d |= uint64_t((lbo >> 4) & 0x3FFF) << 16;
+  d |= uint64_t(1024 >> 4) << 32;
+  d |= uint64_t(1) << 46;
+  d |= uint64_t(2) << 61;  // SWIZZLE_128B
+  return d;
+}
 // Instruction descriptor: kind::tf32, FP32 accumulate, M x N, operand majors.
 __host__ __device__ constexpr uint32_t idesc_tf32(int M, int N, int a_mn_major, int b_mn_major) {
   return (1u << 4)                         // D format F32
          | (2u << 7) | (2u << 10)          // A, B format TF32
+         | (uint32_t(a_mn_major) << 15) | (uint32_t(b_mn_major) << 16) |
+         (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
+}
+
+// The same for kind::f16, both operands fp16 (fmt 0) or both bf16 (fmt 1).
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int a_mn_major, int b_mn_major, int fmt) {
+  return (1u << 4)                                  // D format F32
+         | (uint32_t(fmt) << 7) | (uint32_t(fmt) << 10)  // A, B format
          | (uint32_t(a_mn_major) << 15) | (uint32_t(b_mn_major) << 16) |
          (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
