@@ -11,6 +11,7 @@ rows, the last is the row. A tensor whose rows lie apart (a channel range of a
 wider one) is taken as it is; one that is no matrix of contiguous rows (a
 transpose, an expanded gradient) is copied first.
 """
+import ctypes
 import struct
 
 import torch
@@ -28,59 +29,47 @@ _DENSE_BACKWARD = struct.Struct("<8Q10q2ifi")
 
 
 def _rows(t, what, cols=None):
-    """The tensor as a matrix of rows: (data pointer, rows, columns, row stride, the tensor kept alive)."""
-    c = t.shape[-1] if t.dim() else 0
-    if t.dim() == 2:
-        rows = t.shape[0]
-    else:
-        if t.dim() == 0:
-            raise ValueError("%s: a scalar has no rows" % what)
-        rows = t.numel() // c if c else 0
+    """The tensor as a matrix of rows: (data pointer, rows, columns, row stride, the tensor to keep alive)."""
+    shape = t.shape
+    if not shape:
+        raise ValueError("%s: a scalar has no rows" % what)
+    c = shape[-1]
     if cols is not None and c != cols:
         raise ValueError("%s: rows of %d elements, expected %d" % (what, c, cols))
-    if rows <= 1:
-        if c > 1 and t.stride(-1) != 1:
-            t = t.contiguous()
+    rows = shape[0] if len(shape) == 2 else (t.numel() // c if c else 0)
+    if t.is_contiguous():
         return t.data_ptr(), rows, c, c, t
-    if t.dim() == 2:
-        s = t.stride(0)
-        if (t.stride(1) == 1 or c == 1) and s >= c:
-            return t.data_ptr(), rows, c, s, t
-    elif not t.is_contiguous():
+    if t.stride(-1) == 1 or c == 1:
         # Leading dimensions that step evenly through memory are rows too.
-        lead = [(n, st) for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
-        even = all(a_st == b_n * b_st for (_, a_st), (b_n, b_st) in zip(lead, lead[1:]))
-        if even and (t.stride(-1) == 1 or c == 1) and lead[-1][1] >= c:
-            return t.data_ptr(), rows, c, lead[-1][1], t
+        lead = [(n, st) for n, st in zip(shape[:-1], t.stride()[:-1]) if n != 1]
+        if not lead:
+            return t.data_ptr(), rows, c, c, t
+        step = lead[-1][1]
+        if step >= c and all(a[1] == b[0] * b[1] for a, b in zip(lead, lead[1:])):
+            return t.data_ptr(), rows, c, step, t
     t = t.contiguous()
     return t.data_ptr(), rows, c, c, t
 
 
-def _device(t, *others):
-    if not t.is_cuda:
+def _where(t, *others):
+    """The device index of tensors that must all be on one CUDA device."""
+    device = t.get_device()
+    if device < 0:
         raise ValueError("the operators take CUDA tensors, got one on %s" % t.device)
     for o in others:
-        if o is not None and o.device != t.device:
+        if o is not None and o.get_device() != device:
             raise ValueError("tensors on %s and %s" % (t.device, o.device))
-    return t.device.index
+    return device
 
 
 def _dtype(t, *others):
-    code = _DT.get(t.dtype)
-    if code is None:
-        raise TypeError("the operators take float32, bfloat16 or float16, got %s" % t.dtype)
+    dt = t.dtype
+    if dt not in _DT:
+        raise TypeError("the operators take float32, bfloat16 or float16, got %s" % dt)
     for o in others:
-        if o is not None and o.dtype != t.dtype:
-            raise TypeError("tensors of %s and %s" % (t.dtype, o.dtype))
-    return code
-
-
-def _params(dtype, c, *params):
-    """The type code of the norm's parameter vectors: the tensors' own type, or fp32."""
-    pt = params[0].dtype
-    if pt is not dtype and pt is not torch.float32:
-        raise TypeError("parameters of %s with tensors of %s" % (pt, dtype))
-    return _DT[pt], [_vector(p, pt, c) for p in params]
+        if o is not None and o.dtype is not dt:
+            raise TypeError("tensors of %s and %s" % (dt, o.dtype))
+    return _DT[dt]
 
 
 def _vector(p, dtype, n):
@@ -91,62 +80,97 @@ def _vector(p, dtype, n):
     return p if p.is_contiguous() else p.contiguous()
 
 
-def _launch(entry, query, layout, ws_at, values, device):
+def _param_dtype(p, dtype):
+    """The norm's parameter vectors are of the tensors' own type or fp32."""
+    if p.dtype is not dtype and p.dtype is not torch.float32:
+        raise TypeError("parameters of %s with tensors of %s" % (p.dtype, dtype))
+    return p.dtype
+
+
+def _act(name):
+    if name not in ACTS:
+        raise ValueError("act %r is not one of %s" % (name, ", ".join(ACTS)))
+    return ACTS[name]
+
+
+# Workspaces up to _WS_KEEP bytes stay with their stream: its calls run one
+# after the other, so they can share one. Larger ones, and those of a captured
+# graph (which must own its memory), come from torch's allocator at each call.
+_WS_KEEP = 32 << 20
+_workspaces = {}
+
+
+def _launch(entry, layout, values, device, ws_at=None):
     """Call `entry` on the device's current stream with the packed argument
-    struct, giving it the workspace that `query` asks for."""
+    struct. With `ws_at` (the index of the workspace pointer) it may need a workspace."""
     lib = _native.lib()
     if device != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return _launch(entry, query, layout, ws_at, values, device)
-    if query is not None:
-        need = _native.ctypes.c_int64()
-        rc = getattr(lib, query)(layout.pack(*values), _native.ctypes.byref(need))
-        if rc != 0:
-            _native.check(rc)
-        if need.value:
-            ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
-            values[ws_at] = ws.data_ptr()
-            values[ws_at + 1] = need.value
-    rc = getattr(lib, entry)(layout.pack(*values), torch.cuda.current_stream().cuda_stream)
-    if rc != 0:
+            return _launch(entry, layout, values, device, ws_at)
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if ws_at is not None and not torch.cuda.is_current_stream_capturing():
+        kept = _workspaces.get((device, stream))
+        if kept is not None:
+            values[ws_at], values[ws_at + 1] = kept[1], kept[2]
+    rc = getattr(lib, entry)(layout.pack(*values), stream)
+    if rc == _native.MX_OK:
+        return
+    if rc != _native.MX_E_INVALID or ws_at is None:
         _native.check(rc)
+    # Refused, perhaps only for the workspace: the query refuses too if not.
+    need = ctypes.c_int64()
+    _native.check(getattr(lib, entry + "_workspace")(layout.pack(*values), ctypes.byref(need)))
+    if need.value <= values[ws_at + 1]:
+        _native.check(getattr(lib, entry)(layout.pack(*values), stream))
+    keep = need.value <= _WS_KEEP and not torch.cuda.is_current_stream_capturing()
+    size = max(need.value, 1 << 20) if keep else need.value
+    ws = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", device))
+    if keep:
+        _workspaces[device, stream] = (ws, ws.data_ptr(), size)
+    values[ws_at], values[ws_at + 1] = ws.data_ptr(), size
+    _native.check(getattr(lib, entry)(layout.pack(*values), stream))
 
 
 def layer_norm(x, scale, bias, eps=1e-6, stats=False):
     """(x - mean) * rstd * scale + bias over the last dimension. With `stats`
     also the fp32 mean and rstd of every row, which the backward pass takes:
     (y, mean, rstd). scale and bias are of x's type or fp32."""
-    device, code = _device(x, scale, bias), _dtype(x)
-    xp, rows, c, xs, x_ = _rows(x, "x")
-    pcode, (scale, bias) = _params(x.dtype, c, scale, bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if stats:
-        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _launch("mx_layer_norm", None, _NORM, 0,
-            (xp, scale.data_ptr(), bias.data_ptr(), y.data_ptr(), mean.data_ptr() if stats else 0,
-             rstd.data_ptr() if stats else 0, rows, c, xs, c, code, pcode, eps, 0), device)
-    return (y, mean, rstd) if stats else y
+    device, code = _where(x, scale, bias), _dtype(x)
+    xp, rows, c, xs, x = _rows(x, "x")
+    pt = _param_dtype(scale, x.dtype)
+    scale, bias = _vector(scale, pt, c), _vector(bias, pt, c)
+    shape = x.shape
+    y = x.new_empty(shape)
+    if not stats:
+        _launch("mx_layer_norm", _NORM, (xp, scale.data_ptr(), bias.data_ptr(), y.data_ptr(), 0, 0, rows, c, xs, c,
+                                         code, _DT[pt], eps, 0), device)
+        return y
+    mean = x.new_empty(shape[:-1], dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    _launch("mx_layer_norm", _NORM, (xp, scale.data_ptr(), bias.data_ptr(), y.data_ptr(), mean.data_ptr(),
+                                     rstd.data_ptr(), rows, c, xs, c, code, _DT[pt], eps, 0), device)
+    return y, mean, rstd
 
 
 def layer_norm_backward(dy, x, scale, mean, rstd, need_dx=True, need_params=True):
     """The gradients of layer_norm: (dx, dscale, dbias), None where not needed.
     mean and rstd are the forward pass's."""
-    device, code = _device(x, dy, scale, mean, rstd), _dtype(x, dy)
-    xp, rows, c, xs, x_ = _rows(x, "x")
+    device, code = _where(x, dy, scale, mean, rstd), _dtype(x, dy)
     if dy.shape != x.shape:
         raise ValueError("dy has shape %s, x %s" % (tuple(dy.shape), tuple(x.shape)))
-    dyp, _, _, dys, dy_ = _rows(dy, "dy")
-    pcode, (scale,) = _params(x.dtype, c, scale)
+    xp, rows, c, xs, x = _rows(x, "x")
+    dyp, _, _, dys, dy = _rows(dy, "dy")
+    pt = _param_dtype(scale, x.dtype)
+    scale = _vector(scale, pt, c)
     mean, rstd = _vector(mean, torch.float32, rows), _vector(rstd, torch.float32, rows)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
-    dscale = torch.empty_like(scale) if need_params else None
-    dbias = torch.empty_like(scale) if need_params else None
-    _launch("mx_layer_norm_backward", "mx_layer_norm_backward_workspace" if need_params else None, _NORM_BACKWARD, 8,
+    dx = x.new_empty(x.shape) if need_dx else None
+    dscale = dbias = None
+    if need_params:
+        dscale, dbias = torch.empty_like(scale), torch.empty_like(scale)
+    _launch("mx_layer_norm_backward", _NORM_BACKWARD,
             [dyp, xp, scale.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr() if need_dx else 0,
              dscale.data_ptr() if need_params else 0, dbias.data_ptr() if need_params else 0, 0, 0, rows, c, dys, xs, c,
-             code, pcode], device)
+             code, _DT[pt]], device, 8)
     return dx, dscale, dbias
 
 
@@ -155,57 +179,51 @@ def dense(x, w, bias=None, act="none", slope=0.2, residual=None, save_pre=False)
     [..., n]. act is one of "none", "gelu" (the erf form), "lrelu" (leaky, with
     `slope`), "sigmoid". With `save_pre` also x @ w.T + bias, which the backward
     pass of an activation takes: (y, pre)."""
-    device, code = _device(x, w, bias, residual), _dtype(x, w, bias, residual)
-    xp, m, k, xs, x_ = _rows(x, "x")
+    device, code = _where(x, w, bias, residual), _dtype(x, w, bias, residual)
+    xp, m, k, xs, x = _rows(x, "x")
     if w.dim() != 2:
         raise ValueError("w has %d dimensions, expected 2" % w.dim())
-    wp, n, _, ws, w_ = _rows(w, "w", k)
+    wp, n, _, ws, w = _rows(w, "w", k)
     shape = x.shape[:-1] + (n,)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    pre = torch.empty(shape, dtype=x.dtype, device=x.device) if save_pre else None
-    rp = rs = 0
+    y = x.new_empty(shape)
+    pre = torch.empty_like(y) if save_pre else None
+    rp = rs = bp = 0
     if residual is not None:
         if residual.shape != shape:
             raise ValueError("residual has shape %s, the product %s" % (tuple(residual.shape), tuple(shape)))
-        rp, _, _, rs, r_ = _rows(residual, "residual")
+        rp, _, _, rs, residual = _rows(residual, "residual")
     if bias is not None:
         bias = _vector(bias, x.dtype, n)
-    _launch("mx_dense", "mx_dense_workspace", _DENSE, 6,
-            [xp, wp, 0 if bias is None else bias.data_ptr(), rp, y.data_ptr(), pre.data_ptr() if save_pre else 0, 0, 0,
-             m, k, n, xs, ws, rs, n, n, code, _act(act), slope, 0], device)
+        bp = bias.data_ptr()
+    _launch("mx_dense", _DENSE, [xp, wp, bp, rp, y.data_ptr(), pre.data_ptr() if save_pre else 0, 0, 0, m, k, n, xs,
+                                 ws, rs, n, n, code, _act(act), slope, 0], device, 6)
     return (y, pre) if save_pre else y
 
 
 def dense_backward(dy, x, w, pre=None, act="none", slope=0.2, need_dx=True, need_dw=True, need_db=True):
     """The gradients of dense: (dx, dw, db), None where not needed. pre is the
     forward pass's (with an activation); the residual's gradient is dy."""
-    device, code = _device(dy, x, w, pre), _dtype(dy, x, w, pre)
-    dyp, m, n, dys, dy_ = _rows(dy, "dy")
-    xp, mx, k, xs, x_ = _rows(x, "x")
-    if w.dim() != 2 or w.shape[0] != n:
-        raise ValueError("w has shape %s, dy rows of %d" % (tuple(w.shape), n))
-    wp, _, _, ws, w_ = _rows(w, "w", k)
+    device, code = _where(dy, x, w, pre), _dtype(dy, x, w, pre)
     if dy.shape[:-1] != x.shape[:-1]:
         raise ValueError("dy has shape %s, x %s" % (tuple(dy.shape), tuple(x.shape)))
+    dyp, m, n, dys, dy = _rows(dy, "dy")
+    xp, _, k, xs, x = _rows(x, "x")
+    if w.dim() != 2 or w.shape[0] != n:
+        raise ValueError("w has shape %s, dy rows of %d" % (tuple(w.shape), n))
+    wp, _, _, ws, w = _rows(w, "w", k)
     pp = ps = 0
     if act != "none":
         if pre is None or pre.shape != dy.shape:
             raise ValueError("the gradient of %s needs pre, of dy's shape" % act)
-        pp, _, _, ps, p_ = _rows(pre, "pre")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
-    dw = torch.empty((n, k), dtype=x.dtype, device=x.device) if need_dw else None
-    db = torch.empty(n, dtype=x.dtype, device=x.device) if need_db else None
-    _launch("mx_dense_backward", "mx_dense_backward_workspace", _DENSE_BACKWARD, 7,
+        pp, _, _, ps, pre = _rows(pre, "pre")
+    dx = x.new_empty(x.shape) if need_dx else None
+    dw = x.new_empty((n, k)) if need_dw else None
+    db = x.new_empty((n,)) if need_db else None
+    _launch("mx_dense_backward", _DENSE_BACKWARD,
             [dyp, xp, wp, pp, dx.data_ptr() if need_dx else 0, dw.data_ptr() if need_dw else 0,
-             db.data_ptr() if need_db else 0, 0, 0, m, k, n, dys, xs, ws, ps, k, k, code, _act(act), slope, 0], device)
+             db.data_ptr() if need_db else 0, 0, 0, m, k, n, dys, xs, ws, ps, k, k, code, _act(act), slope, 0], device,
+            7)
     return dx, dw, db
-
-
-def _act(name):
-    code = ACTS.get(name)
-    if code is None:
-        raise ValueError("act %r is not one of %s" % (name, ", ".join(ACTS)))
-    return code
 
 
 def poll():
