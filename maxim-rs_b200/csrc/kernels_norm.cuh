@@ -16,6 +16,7 @@
 // results do not change from run to run).
 #pragma once
 
+#include "gpu_common.cuh"
 #include "kernels_vec.cuh"
 
 namespace mx {
@@ -40,9 +41,9 @@ struct NormBwd {
   int param_f32;
 };
 
-// Sum over the L lanes of a row. For L > 32 the warps' sums meet in `red`
-// (two slots alternate, so one barrier a sum is enough: a warp can only be
-// one sum ahead of another).
+// Sum over the L lanes of a row; every lane gets the sums. For L > 32 the
+// warps' sums meet in `red` (two slots alternate, so one barrier a sum is
+// enough: a warp can only be one sum ahead of another).
 template <int L, int K>
 __device__ __forceinline__ void row_sum(float (&s)[K], float (*red)[32 * K], int& slot) {
 #pragma unroll
@@ -59,12 +60,11 @@ __device__ __forceinline__ void row_sum(float (&s)[K], float (*red)[32 * K], int
       for (int k = 0; k < K; ++k) r[warp * K + k] = s[k];
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      float t = lane < W ? r[lane * K + k] : 0.0f;
+    for (int k = 0; k < K; ++k) s[k] = r[(lane % W) * K + k];
 #pragma unroll
-      for (int o = W / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
-      s[k] = __shfl_sync(0xFFFFFFFFu, t, 0);
-    }
+    for (int o = W / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < K; ++k) s[k] += __shfl_xor_sync(0xFFFFFFFFu, s[k], o);
   }
 }
 
@@ -74,12 +74,65 @@ constexpr int kNormThreads = L <= 32 ? 256 : L;
 template <int V, int NV>
 constexpr bool kNormHold = V * NV <= 16;
 
+// Rows spread over a block go through a ring in shared memory, filled by
+// asynchronous 16-byte copies several rows ahead: every thread copies, waits for
+// and reads its own vectors, so the ring needs no barrier. (One row ahead in
+// registers left too few bytes in flight: 55 us for 16411 x 4096 bf16, 88 us
+// backward.) Short rows, many to a block, have enough in flight in registers.
+template <int V, int L>
+constexpr bool kNormRing = V > 1 && L > 32;
+// Stages of `bytes` each: up to 4 in 64 KB, else 2, else 1 (the next row is
+// on its way while the current one is worked on in registers).
+constexpr int norm_stages(int bytes) { return bytes <= 16384 ? 4 : (bytes <= 65536 ? 2 : 1); }
+template <int V, int L, int NV, int TENSORS>
+constexpr int kNormStages = norm_stages(L * NV * 16 * TENSORS);
+template <int V, int L, int NV, int TENSORS>
+constexpr int kNormSmem = kNormRing<V, L> ? kNormStages<V, L, NV, TENSORS> * L * NV * 16 * TENSORS : 0;
+
+// 16 bytes from src, or 16 zero bytes.
+__device__ __forceinline__ void copy_async16(void* dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src), "r"(on ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Values are worked on in pairs (f32x2: the same roundings at half the
+// instructions; with 2-byte elements the norm is otherwise bound by its
+// instruction issue: 16411 x 4096 bf16 took 57 us in scalar form, 12 us over
+// the memory's time). A thread's single value has a zero beside it.
+template <int E>
+constexpr int kPairs = (E + 1) / 2;
+template <class T, int V, int NV>
+__device__ __forceinline__ void unpack_pairs(const Raw<T, V> (&q)[NV], uint64_t (&v)[kPairs<V * NV>]) {
+  float f[V * NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) raw_unpack<T, V>(q[j], f + j * V);
+#pragma unroll
+  for (int i = 0; i < kPairs<V * NV>; ++i) v[i] = f2_pack(f[2 * i], 2 * i + 1 < V * NV ? f[(2 * i + 1) % (V * NV)] : 0.0f);
+}
+__device__ __forceinline__ float pair_sum(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
+
 template <class T, int V, int L, int NV>
 __global__ void __launch_bounds__(kNormThreads<L>) layer_norm_kernel(NormFwd p) {
-  constexpr int E = V * NV;
+  constexpr int E = V * NV, P = kPairs<E>;
   constexpr bool HOLD = kNormHold<V, NV>;
   constexpr int GROUPS = kNormThreads<L> / L;
-  __shared__ float red[2][32];
+  __shared__ float red[2][64];
   int slot = 0;
   const int lane = threadIdx.x % L;
   const T* x = static_cast<const T*>(p.x);
@@ -88,66 +141,145 @@ __global__ void __launch_bounds__(kNormThreads<L>) layer_norm_kernel(NormFwd p) 
   bool in[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) in[j] = (j * L + lane) * V < p.c;
-  float w[HOLD ? E : 1], b[HOLD ? E : 1];
+  // -m where the pair's values exist, 0 where they do not (those stay 0).
+  auto minus = [&](float m, int i) {
+    const bool a = in[2 * i / V], b = 2 * i + 1 < E && in[(2 * i + 1) % E / V];
+    return f2_pack(a ? -m : 0.0f, b ? -m : 0.0f);
+  };
+  auto param = [&](const void* q, int i) {
+    float f[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = 2 * i + h;
+      f[h] = e < E && in[e % E / V] ? param_at<T>(q, p.param_f32, ((e / V) * L + lane) * V + e % V) : 0.0f;
+    }
+    return f2_pack(f[0], f[1]);
+  };
+  uint64_t w[HOLD ? P : 1], b[HOLD ? P : 1];
   if constexpr (HOLD) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int col = ((i / V) * L + lane) * V + i % V;
-      w[i] = in[i / V] ? param_at<T>(p.scale, p.param_f32, col) : 0.0f;
-      b[i] = in[i / V] ? param_at<T>(p.bias, p.param_f32, col) : 0.0f;
-    }
+    for (int i = 0; i < P; ++i) w[i] = param(p.scale, i), b[i] = param(p.bias, i);
   }
+  // L > 32: the values in this warp and in the warp that this lane stands for below.
+  constexpr int W = L > 32 ? L / 32 : 1;
+  auto warp_values = [&](int k) {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) n += min(max(p.c - (j * L + k * 32) * V, 0), 32 * V);
+    return float(n);
+  };
+  const float n_own = warp_values(threadIdx.x >> 5), n_of = warp_values(threadIdx.x % W);
+  const float inv_own = n_own > 0.0f ? 1.0f / n_own : 0.0f, inv_of = n_of > 0.0f ? 1.0f / n_of : 0.0f;
+
   auto load = [&](int64_t r, Raw<T, V>(&q)[NV]) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       q[j] = r < p.rows && in[j] ? raw_load<T, V>(x + r * p.x_stride + (j * L + lane) * V) : raw_zero<T, V>();
   };
   const int64_t step = int64_t(gridDim.x) * GROUPS;
+  constexpr bool RING = kNormRing<V, L>;
+  constexpr int S = kNormStages<V, L, NV, 1>;
+  extern __shared__ uint4 ring[];
+  auto fill = [&](int64_t r, int stage) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const bool on = r < p.rows && in[j];
+      copy_async16(&ring[(stage * NV + j) * L + lane], on ? x + r * p.x_stride + (j * L + lane) * V : x, on);
+    }
+    copy_commit();
+  };
   Raw<T, V> cur[NV];
-  load(int64_t(blockIdx.x) * GROUPS + threadIdx.x / L, cur);
+  int stage = 0;
+  if constexpr (RING) {
+#pragma unroll
+    for (int k = 0; k < S; ++k) fill(blockIdx.x + k * step, k);
+  } else {
+    load(int64_t(blockIdx.x) * GROUPS + threadIdx.x / L, cur);
+  }
   for (int64_t base = int64_t(blockIdx.x) * GROUPS; base < p.rows; base += step) {
     const int64_t r = base + threadIdx.x / L;
-    Raw<T, V> next[HOLD ? NV : 1];
-    if constexpr (HOLD) load(r + step, next);
-    float v[E], s[1] = {0.0f};
+    Raw<T, V> next[HOLD && !RING ? NV : 1];
+    if constexpr (RING) {
+      copy_wait<S - 1>();
 #pragma unroll
-    for (int j = 0; j < NV; ++j) raw_unpack<T, V>(cur[j], v + j * V);
-#pragma unroll
-    for (int i = 0; i < E; ++i) s[0] += v[i];
-    row_sum<L, 1>(s, red, slot);
-    // Rounded on its own: contracted into the subtractions below it would not be the mean that is stored.
-    const float mean = __fmul_rn(s[0], inv_c);
-    float q[1] = {0.0f};
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      v[i] = in[i / V] ? v[i] - mean : 0.0f;
-      q[0] = fmaf(v[i], v[i], q[0]);
+      for (int j = 0; j < NV; ++j) cur[j] = raw_load<T, V>(reinterpret_cast<const T*>(&ring[(stage * NV + j) * L + lane]));
+      fill(r + S * step, stage);
+      stage = stage + 1 == S ? 0 : stage + 1;
+    } else if constexpr (HOLD) {
+      load(r + step, next);
     }
-    row_sum<L, 1>(q, red, slot);
-    const float rstd = 1.0f / sqrtf(fmaf(q[0], inv_c, p.eps));
+    uint64_t v[P];
+    unpack_pairs<T, V, NV>(cur, v);
+    // The sum, then the squares about a mean: the row's own where its lanes are
+    // in one warp, else the warp's, the warps' squares joined by
+    // sum_w [M2_w + n_w (mean_w - mean)^2], so that a row has one barrier.
+    auto sum = [&] {
+      uint64_t t = v[0];
+#pragma unroll
+      for (int i = 1; i < P; ++i) t = f2_add(t, v[i]);
+      float s = pair_sum(t);
+#pragma unroll
+      for (int o = (L < 32 ? L : 32) / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+      return s;
+    };
+    auto squares = [&](float m, bool keep) {
+      uint64_t t = 0;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const uint64_t d = f2_add(v[i], minus(m, i));
+        t = f2_fma(d, d, t);
+        if (keep) v[i] = d;
+      }
+      float q = pair_sum(t);
+#pragma unroll
+      for (int o = (L < 32 ? L : 32) / 2; o > 0; o >>= 1) q += __shfl_xor_sync(0xFFFFFFFFu, q, o);
+      return q;
+    };
+    float s = sum(), mean, q;
+    if constexpr (L <= 32) {
+      // Rounded on its own: contracted into the subtractions it would not be the mean that is stored.
+      mean = __fmul_rn(s, inv_c);
+      q = squares(mean, true);
+    } else {
+      q = squares(s * inv_own, false);
+      float* part = red[slot];
+      slot ^= 1;
+      if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s, part[32 + (threadIdx.x >> 5)] = q;
+      __syncthreads();
+      const float sw = part[threadIdx.x % W];
+      q = part[32 + threadIdx.x % W];
+      s = sw;
+#pragma unroll
+      for (int o = W / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+      mean = __fmul_rn(s, inv_c);
+      const float d = fmaf(sw, inv_of, -mean);
+      q = fmaf(n_of * d, d, q);
+#pragma unroll
+      for (int o = W / 2; o > 0; o >>= 1) q += __shfl_xor_sync(0xFFFFFFFFu, q, o);
+#pragma unroll
+      for (int i = 0; i < P; ++i) v[i] = f2_add(v[i], minus(mean, i));
+    }
+    const float rstd = 1.0f / sqrtf(fmaf(q, inv_c, p.eps));
     if (r < p.rows) {
       if (lane == 0) {
         if (p.mean) p.mean[r] = mean;
         if (p.rstd) p.rstd[r] = rstd;
       }
+      const uint64_t rr = f2_pack(rstd, rstd);
+      float o[2 * P];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (!in[j]) continue;
-        const int col = (j * L + lane) * V;
-        float o[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float wi = HOLD ? w[HOLD ? j * V + i : 0] : param_at<T>(p.scale, p.param_f32, col + i);
-          const float bi = HOLD ? b[HOLD ? j * V + i : 0] : param_at<T>(p.bias, p.param_f32, col + i);
-          o[i] = fmaf(v[j * V + i] * rstd, wi, bi);
-        }
-        raw_store<T, V>(y + r * p.y_stride + col, raw_pack<T, V>(o));
+      for (int i = 0; i < P; ++i) {
+        const uint64_t wi = HOLD ? w[HOLD ? i : 0] : param(p.scale, i), bi = HOLD ? b[HOLD ? i : 0] : param(p.bias, i);
+        f2_unpack(f2_fma(f2_mul(v[i], rr), wi, bi), o[2 * i], o[2 * i + 1]);
       }
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (in[j]) raw_store<T, V>(y + r * p.y_stride + (j * L + lane) * V, raw_pack<T, V>(o + j * V));
     }
-    if constexpr (HOLD) {
+    if constexpr (HOLD && !RING) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) cur[j] = next[j];
-    } else {
+    } else if constexpr (!RING) {
       load(r + step, cur);
     }
   }
@@ -196,7 +328,7 @@ __global__ void __launch_bounds__(512) layer_norm_long_kernel(NormFwd p) {
 
 template <class T, int V, int L, int NV>
 __global__ void __launch_bounds__(kNormThreads<L>) layer_norm_backward_kernel(NormBwd p) {
-  constexpr int E = V * NV;
+  constexpr int E = V * NV, P = kPairs<E>;
   constexpr bool HOLD = kNormHold<V, NV>;
   constexpr int GROUPS = kNormThreads<L> / L;
   __shared__ float red[2][64];
@@ -208,15 +340,25 @@ __global__ void __launch_bounds__(kNormThreads<L>) layer_norm_backward_kernel(No
   bool in[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) in[j] = (j * L + lane) * V < p.c;
-  float w[HOLD ? E : 1], acc_s[E], acc_b[E];
+  // Without dx the scale does not matter (and may be absent).
+  auto param = [&](int i) {
+    float f[2];
 #pragma unroll
-  for (int i = 0; i < E; ++i) acc_s[i] = acc_b[i] = 0.0f;
+    for (int h = 0; h < 2; ++h) {
+      const int e = 2 * i + h;
+      f[h] = dx && e < E && in[e % E / V] ? param_at<T>(p.scale, p.param_f32, ((e / V) * L + lane) * V + e % V) : 0.0f;
+    }
+    return f2_pack(f[0], f[1]);
+  };
+  // Values past the row's end have dy = 0, so they add nothing anywhere.
+  uint64_t w[HOLD ? P : 1], acc_s[P], acc_b[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) acc_s[i] = acc_b[i] = 0;
   if constexpr (HOLD) {
 #pragma unroll
-    for (int i = 0; i < E; ++i)
-      w[i] = in[i / V] ? param_at<T>(p.scale, p.param_f32, ((i / V) * L + lane) * V + i % V) : 0.0f;
+    for (int i = 0; i < P; ++i) w[i] = param(i);
   }
-  auto load = [&](int64_t r, Raw<T, V>(&q)[NV], Raw<T, V>(&d)[NV], float& mean, float& rstd) {
+  auto load = [&](int64_t r, Raw<T, V>(&q)[NV], Raw<T, V>(&d)[NV]) {
     const bool on = r < p.rows;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -224,76 +366,113 @@ __global__ void __launch_bounds__(kNormThreads<L>) layer_norm_backward_kernel(No
       q[j] = on && in[j] ? raw_load<T, V>(x + r * p.x_stride + col) : raw_zero<T, V>();
       d[j] = on && in[j] ? raw_load<T, V>(dy + r * p.dy_stride + col) : raw_zero<T, V>();
     }
-    // A row past the last has dy = 0 and rstd = 0: it adds nothing.
-    mean = on ? p.mean[r] : 0.0f;
-    rstd = on ? p.rstd[r] : 0.0f;
+  };
+  auto load_stats = [&](int64_t r, float& mean, float& rstd) {
+    mean = r < p.rows ? p.mean[r] : 0.0f;
+    rstd = r < p.rows ? p.rstd[r] : 0.0f;
   };
   const int64_t step = int64_t(gridDim.x) * GROUPS;
-  Raw<T, V> cx[NV], cd[NV];
-  float mean, rstd;
-  load(int64_t(blockIdx.x) * GROUPS + threadIdx.x / L, cx, cd, mean, rstd);
-  for (int64_t base = int64_t(blockIdx.x) * GROUPS; base < p.rows; base += step) {
-    const int64_t r = base + threadIdx.x / L;
-    Raw<T, V> nx[HOLD ? NV : 1], nd[HOLD ? NV : 1];
-    float nmean = 0.0f, nrstd = 0.0f;
-    if constexpr (HOLD) load(r + step, nx, nd, nmean, nrstd);
-    float s[2] = {0.0f, 0.0f};
+  constexpr bool RING = kNormRing<V, L>;
+  constexpr int S = kNormStages<V, L, NV, 2>;
+  extern __shared__ uint4 ring[];
+  // A row's statistics travel with it, fetched by the first lane of every warp
+  // (a row ahead in registers they were the longest wait).
+  __shared__ float2 stats[RING ? S : 1][RING ? L / 32 : 1];
+  auto fill = [&](int64_t r, int stage) {
+    if ((threadIdx.x & 31) == 0 && r < p.rows) {
+      copy_async4(&stats[stage][threadIdx.x >> 5].x, p.mean + r);
+      copy_async4(&stats[stage][threadIdx.x >> 5].y, p.rstd + r);
+    }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      float xv[V], dv[V];
-      raw_unpack<T, V>(cx[j], xv);
-      raw_unpack<T, V>(cd[j], dv);
+      const bool on = r < p.rows && in[j];
+      const int col = (j * L + lane) * V;
+      copy_async16(&ring[(2 * stage * NV + j) * L + lane], on ? x + r * p.x_stride + col : x, on);
+      copy_async16(&ring[((2 * stage + 1) * NV + j) * L + lane], on ? dy + r * p.dy_stride + col : dy, on);
+    }
+    copy_commit();
+  };
+  Raw<T, V> cx[NV], cd[NV];
+  float mean, rstd;
+  int stage = 0;
+  if constexpr (RING) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = j * V + i;
-        const float n = (xv[i] - mean) * rstd;
-        const float we = HOLD ? w[HOLD ? e : 0]
-                              : (in[j] ? param_at<T>(p.scale, p.param_f32, (j * L + lane) * V + i) : 0.0f);
-        if (in[j]) acc_s[e] = fmaf(dv[i], n, acc_s[e]);
-        acc_b[e] += dv[i];
-        const float g = dv[i] * we;
-        s[0] += g;
-        if (in[j]) s[1] = fmaf(g, n, s[1]);
+    for (int k = 0; k < S; ++k) fill(blockIdx.x + k * step, k);
+  } else {
+    load_stats(int64_t(blockIdx.x) * GROUPS + threadIdx.x / L, mean, rstd);
+    load(int64_t(blockIdx.x) * GROUPS + threadIdx.x / L, cx, cd);
+  }
+  for (int64_t base = int64_t(blockIdx.x) * GROUPS; base < p.rows; base += step) {
+    const int64_t r = base + threadIdx.x / L;
+    Raw<T, V> nx[HOLD && !RING ? NV : 1], nd[HOLD && !RING ? NV : 1];
+    float nmean, nrstd;
+    if constexpr (!RING) load_stats(r + step, nmean, nrstd);
+    if constexpr (RING) {
+      copy_wait<S - 1>();
+      __syncwarp();
+      mean = stats[stage][threadIdx.x >> 5].x, rstd = stats[stage][threadIdx.x >> 5].y;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        cx[j] = raw_load<T, V>(reinterpret_cast<const T*>(&ring[(2 * stage * NV + j) * L + lane]));
+        cd[j] = raw_load<T, V>(reinterpret_cast<const T*>(&ring[((2 * stage + 1) * NV + j) * L + lane]));
       }
+      __syncwarp();  // the warp has read the statistics
+      fill(r + S * step, stage);
+      stage = stage + 1 == S ? 0 : stage + 1;
+    } else if constexpr (HOLD) {
+      load(r + step, nx, nd);
+    }
+    const uint64_t mm = f2_pack(-mean, -mean), rr = f2_pack(rstd, rstd);
+    uint64_t n[P], d[P], s0 = 0, s1 = 0;
+    unpack_pairs<T, V, NV>(cx, n);
+    unpack_pairs<T, V, NV>(cd, d);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      n[i] = f2_mul(f2_add(n[i], mm), rr);
+      acc_s[i] = f2_fma(d[i], n[i], acc_s[i]);
+      acc_b[i] = f2_add(acc_b[i], d[i]);
+      d[i] = f2_mul(d[i], HOLD ? w[HOLD ? i : 0] : param(i));
+      s0 = f2_add(s0, d[i]);
+      s1 = f2_fma(d[i], n[i], s1);
     }
     if (dx) {
+      float s[2] = {pair_sum(s0), pair_sum(s1)};
       row_sum<L, 2>(s, red, slot);
-      const float mg = s[0] * inv_c, mgn = s[1] * inv_c;
       if (r < p.rows) {
+        const float mg = s[0] * -inv_c, mgn = s[1] * -inv_c;
+        const uint64_t mg2 = f2_pack(mg, mg), mgn2 = f2_pack(mgn, mgn);
+        float o[2 * P];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          if (!in[j]) continue;
-          float xv[V], dv[V];
-          raw_unpack<T, V>(cx[j], xv);
-          raw_unpack<T, V>(cd[j], dv);
-          const int col = (j * L + lane) * V;
+        for (int i = 0; i < P; ++i)
+          f2_unpack(f2_mul(f2_fma(n[i], mgn2, f2_add(d[i], mg2)), rr), o[2 * i], o[2 * i + 1]);
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float we = HOLD ? w[HOLD ? j * V + i : 0] : param_at<T>(p.scale, p.param_f32, col + i);
-            const float n = (xv[i] - mean) * rstd;
-            xv[i] = rstd * (fmaf(dv[i], we, -mg) - n * mgn);
-          }
-          raw_store<T, V>(dx + r * p.dx_stride + col, raw_pack<T, V>(xv));
-        }
+        for (int j = 0; j < NV; ++j)
+          if (in[j]) raw_store<T, V>(dx + r * p.dx_stride + (j * L + lane) * V, raw_pack<T, V>(o + j * V));
       }
     }
-    if constexpr (HOLD) {
+    if constexpr (HOLD && !RING) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) cx[j] = nx[j], cd[j] = nd[j];
-      mean = nmean, rstd = nrstd;
-    } else {
-      load(r + step, cx, cd, mean, rstd);
+    } else if constexpr (!RING) {
+      load(r + step, cx, cd);
     }
+    if constexpr (!RING) mean = nmean, rstd = nrstd;
   }
   if (!p.part) return;
   float* out = p.part + int64_t(blockIdx.x) * 2 * p.c;
+  float as[2 * P], ab[2 * P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    f2_unpack(acc_s[i], as[2 * i], as[2 * i + 1]);
+    f2_unpack(acc_b[i], ab[2 * i], ab[2 * i + 1]);
+  }
   if constexpr (GROUPS == 1) {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       if (!in[i / V]) continue;
       const int col = ((i / V) * L + lane) * V + i % V;
-      out[col] = acc_s[i];
-      out[p.c + col] = acc_b[i];
+      out[col] = as[i];
+      out[p.c + col] = ab[i];
     }
   } else {
     // The block's groups hold the same columns: lanes of one warp meet by
@@ -305,13 +484,13 @@ __global__ void __launch_bounds__(kNormThreads<L>) layer_norm_backward_kernel(No
     for (int i = 0; i < E; ++i) {
 #pragma unroll
       for (int o = L; o < 32; o <<= 1) {
-        acc_s[i] += __shfl_xor_sync(0xFFFFFFFFu, acc_s[i], o);
-        acc_b[i] += __shfl_xor_sync(0xFFFFFFFFu, acc_b[i], o);
+        as[i] += __shfl_xor_sync(0xFFFFFFFFu, as[i], o);
+        ab[i] += __shfl_xor_sync(0xFFFFFFFFu, ab[i], o);
       }
       if ((threadIdx.x & 31) < L) {
         const int col = ((i / V) * L + lane) * V + i % V;
-        sums[warp][col] = acc_s[i];
-        sums[warp][COLS + col] = acc_b[i];
+        sums[warp][col] = as[i];
+        sums[warp][COLS + col] = ab[i];
       }
     }
     __syncthreads();
@@ -410,12 +589,16 @@ __global__ void __launch_bounds__(32 * R)
   float t = 0.0f;
   if (col < cols) {
     int b = sub;
-    for (; b + 3 * R < nb; b += 4 * R) {
-      const float v0 = part[int64_t(b) * cols + col], v1 = part[int64_t(b + R) * cols + col];
-      const float v2 = part[int64_t(b + 2 * R) * cols + col], v3 = part[int64_t(b + 3 * R) * cols + col];
-      t += (v0 + v1) + (v2 + v3);
+    for (; b + 7 * R < nb; b += 8 * R) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = part[int64_t(b + i * R) * cols + col];
+      t += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
     }
-    for (; b < nb; b += R) t += part[int64_t(b) * cols + col];
+    float v[7];
+#pragma unroll
+    for (int i = 0; i < 7; ++i) v[i] = b + i * R < nb ? part[int64_t(b + i * R) * cols + col] : 0.0f;
+    t += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + v[6]);
   }
   sums[sub][lane] = t;
   __syncthreads();

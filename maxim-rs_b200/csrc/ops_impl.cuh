@@ -33,33 +33,59 @@ inline void check_launch(const char* what) {
 
 // ------------------------------------------------------------- layer norm
 // The lanes a row is spread over (L) and the vectors a lane holds (NV): the
-// fewest lanes that hold the row in 16 values each, up to a warp; past that
-// a warp, then a block with 16 values a thread, then 32. f(L, NV) is called
-// with the choice as integral constants; returns false for rows too long.
+// fewest lanes that hold the row in 8 values each, up to a warp (fewer lanes
+// mean fewer shuffles a row: 448 x 640 rows of 64 fp32 took 32 us with 4 values
+// a lane); past that a warp or a block with 16 values a thread, then 32.
+// (Twice the lanes with 8 values each measured slower: 16411 x 4096 bf16
+// backward 100 us against 77, the reductions cost a warp the same.)
+// f(L, NV) is called with the choice as integral constants; returns false for
+// rows too long.
 template <int V, class F>
 bool with_norm_shape(int c, F&& f) {
-  constexpr int N16 = 16 / V;
+  constexpr int N8 = V < 8 ? 8 / V : 1, N16 = 16 / V;
   const int64_t vecs = ceil_div(c, V);
 #define MX_SHAPE(L, NV)                                                               \
   if (vecs <= int64_t(L) * (NV)) {                                                    \
     f(std::integral_constant<int, L>(), std::integral_constant<int, (NV)>());         \
     return true;                                                                      \
   }
-  MX_SHAPE(1, 1)
-  MX_SHAPE(2, 1)
-  MX_SHAPE(4, 1)
-  MX_SHAPE(8, 1)
-  MX_SHAPE(16, 1)
-  MX_SHAPE(32, 1)
-  if constexpr (N16 >= 4) MX_SHAPE(32, 4)
-  if constexpr (N16 != 4) MX_SHAPE(32, N16)
-  MX_SHAPE(128, N16 / 2)
+  MX_SHAPE(1, N8)
+  MX_SHAPE(2, N8)
+  MX_SHAPE(4, N8)
+  MX_SHAPE(8, N8)
+  MX_SHAPE(16, N8)
+  MX_SHAPE(32, N8)
+  MX_SHAPE(32, N16)
+  MX_SHAPE(128, N8)
   MX_SHAPE(128, N16)
   MX_SHAPE(256, N16)
   MX_SHAPE(512, N16)
   if constexpr (V > 1) MX_SHAPE(512, 2 * N16)
 #undef MX_SHAPE
   return false;
+}
+
+// Blocks of a kernel that one SM holds at once, asked once per kernel and
+// device, with the opt-in for its shared memory.
+template <class K>
+int resident_blocks(K* kernel, int threads, int smem, std::mutex& mu, int (&known)[64]) {
+  int dev = 0;
+  MX_CUDA(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lock(mu);
+  if (!known[dev]) {
+    MX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    MX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&known[dev], kernel, threads, smem));
+  }
+  return std::max(1, known[dev]);
+}
+template <class T, int V, int L, int NV, bool BACKWARD>
+int norm_resident() {
+  static std::mutex mu;
+  static int known[64] = {};
+  if constexpr (BACKWARD)
+    return resident_blocks(layer_norm_backward_kernel<T, V, L, NV>, kNormThreads<L>, kNormSmem<V, L, NV, 2>, mu, known);
+  else
+    return resident_blocks(layer_norm_kernel<T, V, L, NV>, kNormThreads<L>, kNormSmem<V, L, NV, 1>, mu, known);
 }
 
 template <class T, int V>
@@ -69,8 +95,8 @@ void norm_forward_v(const mx_layer_norm_args& a, const OpsDevice& d, cudaStream_
   const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto nv) {
     constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
     constexpr int THREADS = kNormThreads<L>, GROUPS = THREADS / L;
-    const int64_t blocks = std::min<int64_t>(ceil_div(a.rows, GROUPS), int64_t(d.sms) * (1536 / THREADS));
-    layer_norm_kernel<T, V, L, NV><<<unsigned(blocks), THREADS, 0, s>>>(p);
+    const int64_t blocks = std::min<int64_t>(ceil_div(a.rows, GROUPS), int64_t(d.sms) * norm_resident<T, V, L, NV, false>());
+    layer_norm_kernel<T, V, L, NV><<<unsigned(blocks), THREADS, kNormSmem<V, L, NV, 1>, s>>>(p);
   });
   if (!done) layer_norm_long_kernel<T, V><<<unsigned(std::min<int64_t>(a.rows, int64_t(d.sms) * 4)), 512, 0, s>>>(p);
   check_launch("mx_layer_norm");
@@ -91,12 +117,12 @@ bool norm_backward_vec(const mx_layer_norm_backward_args& a) {
 }
 // Blocks of the backward kernel, which is also how many partial rows of the
 // parameter gradients it leaves.
-template <int V>
+template <class T, int V>
 int64_t norm_backward_blocks(const mx_layer_norm_backward_args& a, const OpsDevice& d) {
   int64_t blocks = 0;
-  const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto) {
-    constexpr int L = decltype(l)::value, THREADS = kNormThreads<L>;
-    blocks = std::min<int64_t>(ceil_div(a.rows, THREADS / L), int64_t(d.sms) * (1024 / THREADS));
+  const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto nv) {
+    constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
+    blocks = std::min<int64_t>(ceil_div(a.rows, kNormThreads<L> / L), int64_t(d.sms) * norm_resident<T, V, L, NV, true>());
   });
   if (!done) blocks = std::min<int64_t>(ceil_div(a.rows, 8), std::max<int64_t>(1, d.sms * 4 / ceil_div(a.c, 32 * V)));
   return blocks;
@@ -104,13 +130,13 @@ int64_t norm_backward_blocks(const mx_layer_norm_backward_args& a, const OpsDevi
 
 template <class T, int V>
 void norm_backward_v(const mx_layer_norm_backward_args& a, const OpsDevice& d, cudaStream_t s) {
-  const int64_t blocks = norm_backward_blocks<V>(a, d);
+  const int64_t blocks = norm_backward_blocks<T, V>(a, d);
   float* part = a.dscale || a.dbias ? static_cast<float*>(a.workspace) : nullptr;
   NormBwd p{a.dy, a.x, a.scale, a.mean, a.rstd, a.dx, part, a.rows, a.dy_stride, a.x_stride, a.dx_stride,
             int(a.c), a.param_dtype == MX_DT_F32};
   const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto nv) {
     constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
-    layer_norm_backward_kernel<T, V, L, NV><<<unsigned(blocks), kNormThreads<L>, 0, s>>>(p);
+    layer_norm_backward_kernel<T, V, L, NV><<<unsigned(blocks), kNormThreads<L>, kNormSmem<V, L, NV, 2>, s>>>(p);
   });
   if (!done) {
     // The sums first: dx may overwrite dy.
@@ -138,7 +164,7 @@ void join_columns(const float* part, int64_t nb, int64_t cols, int64_t split, vo
 template <class T>
 int64_t layer_norm_backward_workspace(const mx_layer_norm_backward_args& a, const OpsDevice& d) {
   if (!a.dscale && !a.dbias) return 0;
-  const int64_t blocks = norm_backward_vec<T>(a) ? norm_backward_blocks<kVec<T>>(a, d) : norm_backward_blocks<1>(a, d);
+  const int64_t blocks = norm_backward_vec<T>(a) ? norm_backward_blocks<T, kVec<T>>(a, d) : norm_backward_blocks<T, 1>(a, d);
   return blocks * 2 * a.c * 4;
 }
 
@@ -158,7 +184,7 @@ void layer_norm_backward(const mx_layer_norm_backward_args& a, const OpsDevice& 
     norm_backward_v<T, 1>(a, d, s);
   if (a.dscale || a.dbias)
     join_columns<T>(static_cast<const float*>(a.workspace),
-                    vec ? norm_backward_blocks<kVec<T>>(a, d) : norm_backward_blocks<1>(a, d), 2 * a.c, a.c, a.dscale,
+                    vec ? norm_backward_blocks<T, kVec<T>>(a, d) : norm_backward_blocks<T, 1>(a, d), 2 * a.c, a.c, a.dscale,
                     a.dbias, out_f32, s);
 }
 
