@@ -271,20 +271,28 @@ __global__ void __launch_bounds__(256)
 }
 
 // ------------------------------------------------- the tensor-core product
-// Warp roles (one CTA per SM, persistent over output tiles of 128 x BN):
+// G CTAs (one, or a pair as cta_group::2) compute a tile of 128 G x BN: each
+// loads 128 rows of A and BN / G rows of B and holds 128 accumulator rows. A
+// pair reads every B row into shared memory once for 256 rows of A: the
+// operands' way through shared memory is what bounds the one-CTA form
+// (8192 x 4096 -> 8192 bf16: 482 us with one, PAIRUS with two).
+// One CTA per SM, persistent over the tiles. Warp roles:
 //   warp 0       TMA producer: 128 bytes of K (64 or 32 elements) a stage
-//   warp 1       MMA issuer (one thread)
+//   warp 1       MMA issuer (one thread, of the pair's leader)
 //   warp 2       TMEM owner
 //   warps 4-11   epilogue: TMEM -> registers -> shared memory (transposing, so
 //                that rows leave in 64-byte or longer runs) -> bias,
 //                activation, residual -> memory; two warps per TMEM lane
 //                quarter, each with half the columns
-//   warps 12-19  fp32 only: the TF32 split (as in the executor's kernels:
+//   warps 12-15  fp32 only: the TF32 split (as in the executor's kernels:
 //                the fp32 tile itself is hi, read truncated to TF32; these
 //                warps write lo = x - hi beside it)
 // Two accumulator sets let the epilogue of one tile overlap the products of
-// the next. In fp32 a set is two regions: hi*hi, and the cross terms
-// hi*lo + lo*hi.
+// the next. In fp32 a set is two regions, hi*hi and the cross terms
+// hi*lo + lo*hi, and the epilogue takes a set every kChunk k-blocks and adds
+// it up in registers: the tensor core truncates its accumulator at each MMA,
+// which over a few hundred of them costs more than the products' own rounding
+// (a sum of 1,900 in one set was off by 2.8e-6 of its size, of 256 by CHUNKERR).
 // Every wait is bounded in time; one that runs out records a code in the
 // status word, and the kernel drains its copies and MMAs, frees its TMEM and
 // returns.
@@ -300,25 +308,27 @@ struct DenseMm {
 
 enum : int { kDenseErrProducer = 0x201, kDenseErrSplit, kDenseErrMmaAcc, kDenseErrMmaStage, kDenseErrEpilogue };
 
-template <class T, int BN>
+template <class T, int BN, int G>
 struct DenseCfg {
   static constexpr bool F32 = sizeof(T) == 4;
   static constexpr int BK = 128 / int(sizeof(T));
+  static constexpr int BROWS = BN / G;  // rows of B a CTA loads
   static constexpr int A_BYTES = 128 * 128;
-  static constexpr int B_BYTES = BN * 128;
+  static constexpr int B_BYTES = BROWS * 128;
   static constexpr int STAGE_BYTES = (A_BYTES + B_BYTES) * (F32 ? 2 : 1);
   static constexpr int STAGES = (192 * 1024 / STAGE_BYTES) < 8 ? (192 * 1024 / STAGE_BYTES) : 8;
   static constexpr int SET_COLS = F32 ? 2 * BN : BN;
   static constexpr int TMEM_COLS = 2 * SET_COLS;
+  static constexpr int CHUNK = F32 ? 8 : 1 << 30;  // k-blocks a set accumulates
   static constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
-  static constexpr int SPLIT_WARP0 = 12, SPLIT_WARPS = F32 ? 8 : 0;
+  static constexpr int SPLIT_WARP0 = 12, SPLIT_WARPS = F32 ? 4 : 0;
   static constexpr int THREADS = 32 * (SPLIT_WARP0 + SPLIT_WARPS);
   // Per epilogue warp 32 rows x 32 floats; 16-byte chunk j of row r lies at
   // j ^ (r & 7), so that neither the writes (a lane a row) nor the reads (four
   // lanes a row) meet in a bank.
   static constexpr int STAGING_BYTES = EPI_WARPS * 4096;
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + STAGING_BYTES + 8 * (3 * STAGES + 5) + 16;
-  static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
+  static_assert(SMEM_BYTES <= 232448 - 64, "shared memory per CTA");
   static_assert(TMEM_COLS <= 512, "TMEM columns");
 };
 
@@ -338,10 +348,41 @@ __device__ __forceinline__ float dense_residual(float v) {
   return __uint_as_float(__float_as_uint(__fsub_rn(v, hi)) + 0x1000u);
 }
 
-template <class T, bool A_MN, bool B_MN, int BN>
-__global__ void __launch_bounds__(DenseCfg<T, BN>::THREADS, 1)
+// A warp's 32 rows x 32 columns of sums, a row in each lane's v: through the
+// staging buffer into rows of 8 columns a lane, and out.
+template <class T>
+__device__ __forceinline__ void dense_store32(const DenseMm& p, float4* st, const float* v, int lane, int split,
+                                              int64_t row0, int64_t col0) {
+  __syncwarp();  // the buffer's last reads
+#pragma unroll
+  for (int i = 0; i < 32; i += 4)
+    st[lane * 8 + ((i / 4) ^ (lane & 7))] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  __syncwarp();
+  const int64_t col = col0 + (lane & 3) * 8;
+  const int valid = int(p.n - col < 8 ? p.n - col : 8);
+  float bias[8];
+  if (!p.epi.part) load_bias<T>(p.epi, col, valid, bias);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
+    const int64_t row = row0 + r;
+    const float4 lo = st[r * 8 + ((2 * (lane & 3)) ^ (r & 7))];
+    const float4 hi = st[r * 8 + ((2 * (lane & 3) + 1) ^ (r & 7))];
+    if (row >= p.m || valid <= 0) continue;
+    if (p.epi.part) {
+      float4* o = reinterpret_cast<float4*>(p.epi.part + (int64_t(split) * p.m + row) * p.epi.ldp + col);
+      o[0] = lo, o[1] = hi;
+    } else {
+      float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      dense_finish<T>(p.epi, x, bias, row, col, valid);
+    }
+  }
+}
+
+template <class T, bool A_MN, bool B_MN, int BN, int G>
+__global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
     dense_mm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, DenseMm p) {
-  using C = DenseCfg<T, BN>;
+  using C = DenseCfg<T, BN, G>;
   using namespace sm100;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -358,17 +399,19 @@ __global__ void __launch_bounds__(DenseCfg<T, BN>::THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = p.tiles_m * p.tiles_n;
   const int items = tiles * p.splits;
+  const uint32_t rank = G == 2 ? cluster_rank() : 0;
+  const int first = blockIdx.x / G, step = gridDim.x / G;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
-      mbar_init(&lo_ready[s], 32 * (C::F32 ? C::SPLIT_WARPS : 1));
+      mbar_init(&lo_ready[s], G * (C::F32 ? C::SPLIT_WARPS : 1));
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 32 * C::EPI_WARPS);
+      mbar_init(&acc_empty[a], G * C::EPI_WARPS);
     }
     mbar_init(drained, 1);
     fence_mbar_init();
@@ -376,11 +419,16 @@ __global__ void __launch_bounds__(DenseCfg<T, BN>::THREADS, 1)
     tma_prefetch(&tmB);
   }
   if (warp == 2) {
-    tmem_alloc(tmem_slot, C::TMEM_COLS);
-    tmem_relinquish();
+    if constexpr (G == 2) {
+      tmem_alloc_pair(tmem_slot, C::TMEM_COLS);
+    } else {
+      tmem_alloc(tmem_slot, C::TMEM_COLS);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (G == 2) cluster_sync_all();  // the barriers of both exist
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   auto fail = [&](int code) {
@@ -391,50 +439,76 @@ __global__ void __launch_bounds__(DenseCfg<T, BN>::THREADS, 1)
     k0 = split * p.kb_split;
     k1 = min(p.kb, k0 + p.kb_split);
   };
+  // Waits on barriers that both CTAs of a pair arrive on, and arrivals on the leader's.
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return G == 2 ? mbar_wait_cluster(bar, parity, vabort) : mbar_wait(bar, parity, vabort);
+  };
+  auto arrive_leader = [&](uint64_t* bar) {
+    if constexpr (G == 2)
+      mbar_arrive_cluster(map_rank(bar, 0));
+    else
+      mbar_arrive(bar);
+  };
+  auto commit = [&](uint64_t* bar) {
+    if constexpr (G == 2)
+      mma_commit_pair(bar);
+    else
+      mma_commit(bar);
+  };
 
   if (warp == 0) {
     if (lane == 0) {
       uint32_t it = 0;
-      for (int w = blockIdx.x; w < items && !*vabort; w += gridDim.x) {
+      for (int w = first; w < items && !*vabort; w += step) {
         int tm, tn, k0, k1;
         dense_tile(p, w % tiles, tm, tn);
         kb_range(w / tiles, k0, k1);
+        const int row = (tm * G + rank) * 128, col = tn * BN + rank * C::BROWS;
         for (int kb = k0; kb < k1; ++kb, ++it) {
           const int s = it % C::STAGES;
-          if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, vabort)) {
+          if (!wait(&empty[s], ((it / C::STAGES) & 1) ^ 1)) {
             fail(kDenseErrProducer);
             break;
           }
           uint8_t* a = base + s * C::STAGE_BYTES;
           uint8_t* b = a + C::A_BYTES;
-          mbar_arrive_expect_tx(&full[s], C::A_BYTES + C::B_BYTES);
-          // K-major: one box of 128 (BN) rows x 128 bytes of K. MN-major: a box
+          // 16-bit pair: both CTAs' bytes count on the leader's barrier, which
+          // the MMA issuer waits on. In fp32 each CTA's split warps wait on
+          // their own.
+          constexpr bool SHARED = G == 2 && !C::F32;
+          if (!SHARED || rank == 0) mbar_arrive_expect_tx(&full[s], (SHARED ? 2 : 1) * (C::A_BYTES + C::B_BYTES));
+          const uint32_t leader_full = SHARED ? map_rank(&full[s], 0) : 0;
+          auto load = [&](uint8_t* dst, const CUtensorMap* map, int c0, int c1) {
+            if constexpr (SHARED)
+              tma_load_2d_pair(dst, map, leader_full, c0, c1);
+            else
+              tma_load_2d(dst, map, &full[s], c0, c1);
+          };
+          // K-major: one box of the tile's rows x 128 bytes of K. MN-major: a box
           // of BK rows of K x 128 bytes of M (N) for each 128 bytes of it.
           if (A_MN) {
 #pragma unroll
-            for (int c = 0; c < 128 / C::BK; ++c)
-              tma_load_2d(a + c * C::BK * 128, &tmA, &full[s], tm * 128 + c * C::BK, kb * C::BK);
+            for (int c = 0; c < 128 / C::BK; ++c) load(a + c * C::BK * 128, &tmA, row + c * C::BK, kb * C::BK);
           } else {
-            tma_load_2d(a, &tmA, &full[s], kb * C::BK, tm * 128);
+            load(a, &tmA, kb * C::BK, row);
           }
           if (B_MN) {
 #pragma unroll
-            for (int c = 0; c < BN / C::BK; ++c)
-              tma_load_2d(b + c * C::BK * 128, &tmB, &full[s], tn * BN + c * C::BK, kb * C::BK);
+            for (int c = 0; c < C::BROWS / C::BK; ++c) load(b + c * C::BK * 128, &tmB, col + c * C::BK, kb * C::BK);
           } else {
-            tma_load_2d(b, &tmB, &full[s], kb * C::BK, tn * BN);
+            load(b, &tmB, kb * C::BK, col);
           }
         }
       }
       if (*vabort)  // copies in flight land before the CTA may leave
         for (uint32_t j = it < C::STAGES ? 0 : it - C::STAGES; j < it; ++j)
-          mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, nullptr);
+          if ((G == 2 && !C::F32 && rank != 0) || !wait(&full[j % C::STAGES], (j / C::STAGES) & 1)) break;
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       constexpr uint32_t idesc =
-          C::F32 ? idesc_tf32(128, BN, A_MN, B_MN)
-                 : idesc_f16(128, BN, A_MN, B_MN, std::is_same<T, __nv_bfloat16>::value ? 1 : 0);
+          C::F32 ? idesc_tf32(128 * G, BN, A_MN, B_MN)
+                 : idesc_f16(128 * G, BN, A_MN, B_MN, std::is_same<T, __nv_bfloat16>::value ? 1 : 0);
       // Steps of one MMA along K, in the descriptors' 16-byte units: 32 bytes
       // of a K-major row, or 16 (8 in fp32) 128-byte rows of an MN-major tile.
       constexpr uint32_t step_a = A_MN ? (C::F32 ? 64u : 128u) : 2u;
@@ -443,21 +517,39 @@ __global__ void __launch_bounds__(DenseCfg<T, BN>::THREADS, 1)
         if (!mn) return desc_kmajor_sw128(addr);
         return C::F32 ? desc_mnmajor_sw128_32b(addr, C::BK * 128) : desc_mnmajor_sw128(addr, C::BK * 128);
       };
+      auto mma = [](uint32_t d, uint64_t da, uint64_t db, uint32_t more) {
+        if constexpr (C::F32) {
+          if constexpr (G == 2)
+            mma_tf32_pair(d, da, db, idesc, more);
+          else
+            mma_tf32(d, da, db, idesc, more);
+        } else {
+          if constexpr (G == 2)
+            mma_f16_pair(d, da, db, idesc, more);
+          else
+            mma_f16(d, da, db, idesc, more);
+        }
+      };
       uint32_t it = 0, tc = 0;
-      for (int w = blockIdx.x; w < items && !*vabort; w += gridDim.x, ++tc) {
+      bool ok = true;
+      for (int w = first; w < items && ok && !*vabort; w += step) {
         int k0, k1;
         kb_range(w / tiles, k0, k1);
-        const uint32_t acc = tc & 1;
-        if (!mbar_wait(&acc_empty[acc], ((tc >> 1) & 1) ^ 1, vabort)) {
-          fail(kDenseErrMmaAcc);
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d = tmem + acc * C::SET_COLS;
-        bool ok = true;
+        uint32_t d = 0;
         for (int kb = k0; kb < k1; ++kb, ++it) {
+          const bool fresh = (kb - k0) % C::CHUNK == 0;
+          if (fresh) {
+            const uint32_t acc = tc & 1;
+            if (!wait(&acc_empty[acc], ((tc >> 1) & 1) ^ 1)) {
+              fail(kDenseErrMmaAcc);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            d = tmem + acc * C::SET_COLS;
+          }
           const int s = it % C::STAGES;
-          if (!mbar_wait(C::F32 ? &lo_ready[s] : &full[s], (it / C::STAGES) & 1, vabort)) {
+          if (!wait(C::F32 ? &lo_ready[s] : &full[s], (it / C::STAGES) & 1)) {
             fail(kDenseErrMmaStage);
             ok = false;
             break;
@@ -470,113 +562,121 @@ __global__ void __launch_bounds__(DenseCfg<T, BN>::THREADS, 1)
             const uint64_t dal = desc(alo, A_MN), dbl = desc(blo, B_MN);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const uint32_t more = kb > k0 || k > 0;
-              mma_tf32(d, da + step_a * k, db + step_b * k, idesc, more);
-              mma_tf32(d + BN, da + step_a * k, dbl + step_b * k, idesc, more);
-              mma_tf32(d + BN, dal + step_a * k, db + step_b * k, idesc, 1u);
+              const uint32_t more = !fresh || k > 0;
+              mma(d, da + step_a * k, db + step_b * k, more);
+              mma(d + BN, da + step_a * k, dbl + step_b * k, more);
+              mma(d + BN, dal + step_a * k, db + step_b * k, 1u);
             }
           } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma_f16(d, da + step_a * k, db + step_b * k, idesc, kb > k0 || k > 0);
+            for (int k = 0; k < 4; ++k) mma(d, da + step_a * k, db + step_b * k, !fresh || k > 0);
           }
-          mma_commit(&empty[s]);
+          commit(&empty[s]);
+          if ((kb - k0) % C::CHUNK == C::CHUNK - 1 || kb == k1 - 1) commit(&acc_full[tc++ & 1]);
         }
-        if (!ok) break;
-        mma_commit(&acc_full[acc]);
       }
       if (*vabort) {
-        mma_commit(drained);
-        mbar_wait(drained, 0, nullptr);
+        commit(drained);
+        wait(drained, 0);
       }
     }
   } else if (warp >= C::EPI_WARP0 && warp < C::EPI_WARP0 + C::EPI_WARPS) {
     const int ew = warp - C::EPI_WARP0, q = warp & 3, half = ew >> 2;
     float4* st = reinterpret_cast<float4*>(staging + ew * 1024);
     uint32_t tc = 0;
-    for (int w = blockIdx.x; w < items && !*vabort; w += gridDim.x, ++tc) {
-      int tm, tn;
+    bool ok = true;
+    for (int w = first; w < items && ok; w += step) {
+      int tm, tn, k0, k1;
       dense_tile(p, w % tiles, tm, tn);
       const int split = w / tiles;
-      const uint32_t acc = tc & 1;
+      kb_range(split, k0, k1);
+      const int64_t row0 = (int64_t(tm) * G + rank) * 128 + q * 32;
+      const int64_t col0 = int64_t(tn) * BN + half * (BN / 2);
       // The warp decides as one: the TMEM loads below need all its lanes.
-      if (!__all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[acc], (tc >> 1) & 1, vabort))) {
-        if (lane == 0) fail(kDenseErrEpilogue);
-        break;
-      }
-      tc_fence_after();
-      const uint32_t d = tmem + (uint32_t(q * 32) << 16) + acc * C::SET_COLS + half * (BN / 2);
-#pragma unroll 1
-      for (int c0 = 0; c0 < BN / 2; c0 += 32) {
-        float v[32];
-        tmem_ld32(d + c0, v);
-        if constexpr (C::F32) {
-          float u[32];
-          tmem_ld32(d + BN + c0, u);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] += u[i];
-        }
-        if (c0 + 32 == BN / 2) {  // the accumulators are read: the next tile may have them
-          tc_fence_before();
-          mbar_arrive(&acc_empty[acc]);
-        }
-#pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          st[lane * 8 + ((i / 4) ^ (lane & 7))] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      auto take = [&] {
+        const bool got = __all_sync(0xFFFFFFFFu, wait(&acc_full[tc & 1], (tc >> 1) & 1));
+        if (!got && lane == 0) fail(kDenseErrEpilogue);
+        tc_fence_after();
+        return got;
+      };
+      auto give = [&] {  // the set is read: the next products may have it
+        tc_fence_before();
         __syncwarp();
-        const int64_t col = int64_t(tn) * BN + half * (BN / 2) + c0 + (lane & 3) * 8;
-        const int valid = int(p.n - col < 8 ? p.n - col : 8);
-        float bias[8];
-        if (!p.epi.part) load_bias<T>(p.epi, col, valid, bias);
+        if (lane == 0) arrive_leader(&acc_empty[tc & 1]);
+        ++tc;
+      };
+      if constexpr (C::F32) {
+        constexpr int COLS = BN / 2;
+        float sum[COLS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = i * 8 + (lane >> 2);
-          const int64_t row = int64_t(tm) * 128 + q * 32 + r;
-          const float4 lo = st[r * 8 + ((2 * (lane & 3)) ^ (r & 7))];
-          const float4 hi = st[r * 8 + ((2 * (lane & 3) + 1) ^ (r & 7))];
-          if (row >= p.m || valid <= 0) continue;
-          if (p.epi.part) {
-            float4* o = reinterpret_cast<float4*>(p.epi.part + (int64_t(split) * p.m + row) * p.epi.ldp + col);
-            o[0] = lo, o[1] = hi;
-          } else {
-            float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-            dense_finish<T>(p.epi, x, bias, row, col, valid);
+        for (int i = 0; i < COLS; ++i) sum[i] = 0.0f;
+        for (int kb = k0; kb < k1 && ok; kb += C::CHUNK) {
+          ok = take();
+          if (!ok) break;
+          const uint32_t d = tmem + (uint32_t(q * 32) << 16) + (tc & 1) * C::SET_COLS + half * COLS;
+#pragma unroll
+          for (int c = 0; c < COLS; c += 16) {
+            float hh[16], cross[16];
+            tmem_ld16x2(d + c, d + BN + c, hh, cross);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[c + i] += hh[i] + cross[i];
           }
+          give();
         }
-        __syncwarp();
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < COLS; c += 32) dense_store32<T>(p, st, sum + c, lane, split, row0, col0 + c);
+      } else {
+        ok = take();
+        if (!ok) break;
+        const uint32_t d = tmem + (uint32_t(q * 32) << 16) + (tc & 1) * C::SET_COLS + half * (BN / 2);
+#pragma unroll 1
+        for (int c = 0; c < BN / 2; c += 32) {
+          float v[32];
+          tmem_ld32(d + c, v);
+          if (c + 32 == BN / 2) give();
+          dense_store32<T>(p, st, v, lane, split, row0, col0 + c);
+        }
       }
     }
   } else if (C::F32 && warp >= C::SPLIT_WARP0) {
     const int tid = threadIdx.x - 32 * C::SPLIT_WARP0;
     uint32_t it = 0;
-    for (int w = blockIdx.x; w < items && !*vabort; w += gridDim.x) {
+    bool ok = true;
+    for (int w = first; w < items && ok; w += step) {
       int k0, k1;
       kb_range(w / tiles, k0, k1);
-      bool ok = true;
       for (int kb = k0; kb < k1; ++kb, ++it) {
         const int s = it % C::STAGES;
-        if (!mbar_wait(&full[s], (it / C::STAGES) & 1, vabort)) {
-          fail(kDenseErrSplit);
-          ok = false;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&full[s], (it / C::STAGES) & 1, vabort));
+        if (!ok) {
+          if (lane == 0) fail(kDenseErrSplit);
           break;
         }
         // Elementwise, so the swizzled layouts do not matter.
         const float4* src = reinterpret_cast<const float4*>(base + s * C::STAGE_BYTES) + tid;
         float4* dst = reinterpret_cast<float4*>(base + s * C::STAGE_BYTES + C::A_BYTES + C::B_BYTES) + tid;
-#pragma unroll 4
-        for (int i = 0; i < (C::A_BYTES + C::B_BYTES) / 16; i += 256) {
+#pragma unroll 8
+        for (int i = 0; i < (C::A_BYTES + C::B_BYTES) / 16; i += 32 * C::SPLIT_WARPS) {
           const float4 v = src[i];
           dst[i] = make_float4(dense_residual(v.x), dense_residual(v.y), dense_residual(v.z), dense_residual(v.w));
         }
         fence_proxy_async_smem();
-        mbar_arrive(&lo_ready[s]);
+        __syncwarp();
+        if (lane == 0) arrive_leader(&lo_ready[s]);
       }
-      if (!ok) break;
     }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (G == 2) cluster_sync_all();  // neither leaves while the other's MMAs, copies or arrivals need it
   tc_fence_after();
-  if (warp == 2) tmem_dealloc(tmem, C::TMEM_COLS);
+  if (warp == 2) {
+    if constexpr (G == 2)
+      tmem_dealloc_pair(tmem, C::TMEM_COLS);
+    else
+      tmem_dealloc(tmem, C::TMEM_COLS);
+  }
 }
 
 }  // namespace mx

@@ -198,36 +198,42 @@ struct Operand {
 };
 
 struct MmPlan {
-  int bn;
+  int bn, g;
   int splits, kb, kb_split;
   int64_t part_bytes;
 };
 
-// Tile width and number of splits of K: the cheapest by a model of the
-// kernel's time, in units of one SM's cycles. A k-block (128 bytes of K) of a
-// 128 x BN tile costs about kStep[BN] cycles, a tile's first loads and last
-// epilogue about 3000; the CTAs of the slowest SM are what counts. Split
-// sums cost their write and reading back (about 2000 bytes a cycle for the
-// whole GPU) and another launch (about 4000).
+// Tile and number of splits of K: the cheapest by a model of the kernel's
+// time, in one SM's cycles. A k-block (128 bytes of K) of a tile costs `step`
+// cycles, a tile's first loads and last epilogue about 3000; the CTAs of the
+// slowest SM are what counts. Split sums cost their write and reading back
+// (about 2000 bytes a cycle for the whole GPU) and another launch (about 4000).
 template <class T>
 MmPlan plan_mm(int64_t m, int64_t n, int64_t k, int sms) {
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int BK = 128 / int(sizeof(T));
+  struct Tile {
+    int bn, g;
+    double step;
+  };
+  constexpr Tile kF32[] = {{64, 1, 1000}, {128, 1, 1500}, {128, 2, 1200}};
+  constexpr Tile k16[] = {{64, 1, 250}, {128, 1, 330}, {256, 1, 620}, {256, 2, 540}};
   MmPlan best{};
   double best_cost = 0;
   const int kb = int(ceil_div(k, BK));
-  for (int bn = 64; bn <= (F32 ? 128 : 256); bn *= 2) {
-    const int64_t tiles = ceil_div(m, 128) * ceil_div(n, bn);
-    const double step = F32 ? (bn == 64 ? 1000 : 1500) : (bn == 64 ? 250 : (bn == 128 ? 330 : 560));
+  for (int i = 0; i < (F32 ? 3 : 4); ++i) {
+    const Tile& t = F32 ? kF32[i % 3] : k16[i];
+    const int64_t tiles = ceil_div(m, 128 * t.g) * ceil_div(n, t.bn);
+    const int workers = sms / t.g;
     for (int want = 1; want <= kb; want = want < 8 ? want + 1 : want * 5 / 4) {
-      if (want > 1 && tiles * want > int64_t(sms) * 2) break;
+      if (want > 1 && tiles * want > int64_t(workers) * 2) break;
       const int per = int(ceil_div(kb, want)), splits = int(ceil_div(kb, per));
-      const int64_t waves = ceil_div(tiles * splits, sms);
-      double cost = double(waves) * (per * step + 1000) + 3000;
+      const int64_t waves = ceil_div(tiles * splits, workers);
+      double cost = double(waves) * (per * t.step + 1000) + 3000;
       if (splits > 1) cost += 4000 + double(splits) * double(m) * double(n) * 8 / 2000;
       if (best.bn == 0 || cost < best_cost) {
         best_cost = cost;
-        best = {bn, splits, kb, per, splits > 1 ? int64_t(splits) * m * round_up(n, 8) * 4 : 0};
+        best = {t.bn, t.g, splits, kb, per, splits > 1 ? int64_t(splits) * m * round_up(n, 8) * 4 : 0};
       }
     }
   }
@@ -256,13 +262,13 @@ CUtensorMap operand_map(const Operand& o, int64_t rows, int64_t cols, int box_ro
   return m;
 }
 
-template <class T, bool A_MN, bool B_MN, int BN>
+template <class T, bool A_MN, bool B_MN, int BN, int G>
 void launch_mm(const Operand& a, const Operand& b, const DenseMm& p, int64_t k, const OpsDevice& d, cudaStream_t s) {
-  using C = DenseCfg<T, BN>;
+  using C = DenseCfg<T, BN, G>;
   constexpr int kMaxDevices = 64;
   static std::mutex mu;
   static bool opted[kMaxDevices] = {};
-  auto* kernel = dense_mm_kernel<T, A_MN, B_MN, BN>;
+  auto* kernel = dense_mm_kernel<T, A_MN, B_MN, BN, G>;
   {
     int dev = 0;
     MX_CUDA(cudaGetDevice(&dev));
@@ -273,10 +279,19 @@ void launch_mm(const Operand& a, const Operand& b, const DenseMm& p, int64_t k, 
     }
   }
   const CUtensorMap ta = A_MN ? operand_map<T>(a, k, p.m, C::BK) : operand_map<T>(a, p.m, k, 128);
-  const CUtensorMap tb = B_MN ? operand_map<T>(b, k, p.n, C::BK) : operand_map<T>(b, p.n, k, BN);
+  const CUtensorMap tb = B_MN ? operand_map<T>(b, k, p.n, C::BK) : operand_map<T>(b, p.n, k, C::BROWS);
   const int64_t items = int64_t(p.tiles_m) * p.tiles_n * p.splits;
-  kernel<<<unsigned(std::min<int64_t>(items, d.sms)), C::THREADS, C::SMEM_BYTES, s>>>(ta, tb, p);
-  check_launch("dense product");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>(items, d.sms / G) * G));
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = G, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = G == 2 ? 1 : 0;
+  MX_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, p));
 }
 
 // D = A B^T with the epilogue `epi`: the product, and the join of its splits.
@@ -286,16 +301,18 @@ void run_mm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64_t k,
   DenseMm p{};
   p.m = m, p.n = n;
   p.kb = plan.kb, p.kb_split = plan.kb_split, p.splits = plan.splits;
-  p.tiles_m = int(ceil_div(m, 128)), p.tiles_n = int(ceil_div(n, plan.bn));
+  p.tiles_m = int(ceil_div(m, 128 * plan.g)), p.tiles_n = int(ceil_div(n, plan.bn));
   p.epi = epi;
   p.status = d.status;
   if (plan.splits > 1) p.epi.part = static_cast<float*>(part), p.epi.ldp = round_up(n, 8);
   auto by_width = [&](auto amn, auto bmn) {
     constexpr bool A = decltype(amn)::value, B = decltype(bmn)::value;
-    if (plan.bn == 64) return launch_mm<T, A, B, 64>(a, b, p, k, d, s);
+    constexpr int WIDE = sizeof(T) == 4 ? 128 : 256;
+    if (plan.g == 2) return launch_mm<T, A, B, WIDE, 2>(a, b, p, k, d, s);
+    if (plan.bn == 64) return launch_mm<T, A, B, 64, 1>(a, b, p, k, d, s);
     if constexpr (sizeof(T) == 2)
-      if (plan.bn == 256) return launch_mm<T, A, B, 256>(a, b, p, k, d, s);
-    launch_mm<T, A, B, 128>(a, b, p, k, d, s);
+      if (plan.bn == 256) return launch_mm<T, A, B, 256, 1>(a, b, p, k, d, s);
+    launch_mm<T, A, B, 128, 1>(a, b, p, k, d, s);
   };
   if (a.mn_major)
     by_width(std::true_type(), std::true_type());
