@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(256)
 // (8192 x 4096 -> 8192 bf16: 482 us with one, PAIRUS with two).
 // One CTA per SM, persistent over the tiles. Warp roles:
 //   warp 0       TMA producer: 128 bytes of K (64 or 32 elements) a stage
-//   warp 1       MMA issuer (one thread, of the pair's leader)
+//   warp 1       MMA issuer (one lane, of the pair's leader)
 //   warp 2       TMEM owner
 //   warps 4-11   epilogue: TMEM -> registers -> shared memory (transposing, so
 //                that rows leave in 64-byte or longer runs) -> bias,
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   __shared__ int abort_flag;
   const volatile int* vabort = &abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int tiles = p.tiles_m * p.tiles_n;
   const int items = tiles * p.splits;
   const uint32_t rank = G == 2 ? cluster_rank() : 0;
@@ -439,10 +439,13 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
     k0 = split * p.kb_split;
     k1 = min(p.kb, k0 + p.kb_split);
   };
-  // Waits on barriers that both CTAs of a pair arrive on, and arrivals on the leader's.
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
+  // Waits for what threads of both CTAs of a pair have arrived on, and those
+  // arrivals, on the leader's barrier. Copies and MMAs complete on a barrier
+  // without a thread's writes to acquire: the plain wait.
+  auto wait_pair = [&](uint64_t* bar, uint32_t parity) {
     return G == 2 ? mbar_wait_cluster(bar, parity, vabort) : mbar_wait(bar, parity, vabort);
   };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, vabort); };
   auto arrive_leader = [&](uint64_t* bar) {
     if constexpr (G == 2)
       mbar_arrive_cluster(map_rank(bar, 0));
@@ -505,7 +508,9 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
           if ((G == 2 && !C::F32 && rank != 0) || !wait(&full[j % C::STAGES], (j / C::STAGES) & 1)) break;
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    // The whole warp runs the loop, so that what the MMAs take is the same in
+    // all lanes and stays in uniform registers; one lane issues.
+    if (rank == 0) {
       constexpr uint32_t idesc =
           C::F32 ? idesc_tf32(128 * G, BN, A_MN, B_MN)
                  : idesc_f16(128 * G, BN, A_MN, B_MN, std::is_same<T, __nv_bfloat16>::value ? 1 : 0);
@@ -530,53 +535,61 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
             mma_f16(d, da, db, idesc, more);
         }
       };
-      uint32_t it = 0, tc = 0;
+      const uint32_t base_u = smem_u32(base);
+      uint32_t s = 0, ph = 0, tc = 0;
       bool ok = true;
-      for (int w = first; w < items && ok && !*vabort; w += step) {
+      for (int w = first; w < items && ok; w += step) {
         int k0, k1;
         kb_range(w / tiles, k0, k1);
         uint32_t d = 0;
-        for (int kb = k0; kb < k1; ++kb, ++it) {
-          const bool fresh = (kb - k0) % C::CHUNK == 0;
+        int left = 0;  // k-blocks the accumulator set still takes
+        for (int kb = k0; kb < k1; ++kb) {
+          const bool fresh = left == 0;
           if (fresh) {
             const uint32_t acc = tc & 1;
-            if (!wait(&acc_empty[acc], ((tc >> 1) & 1) ^ 1)) {
-              fail(kDenseErrMmaAcc);
-              ok = false;
+            ok = __all_sync(0xFFFFFFFFu, wait_pair(&acc_empty[acc], ((tc >> 1) & 1) ^ 1));
+            if (!ok) {
+              if (lane == 0) fail(kDenseErrMmaAcc);
               break;
             }
-            tc_fence_after();
             d = tmem + acc * C::SET_COLS;
+            left = min(C::CHUNK, k1 - kb);
           }
-          const int s = it % C::STAGES;
-          if (!wait(C::F32 ? &lo_ready[s] : &full[s], (it / C::STAGES) & 1)) {
-            fail(kDenseErrMmaStage);
-            ok = false;
+          ok = __all_sync(0xFFFFFFFFu, C::F32 ? wait_pair(&lo_ready[s], ph) : wait(&full[s], ph));
+          if (!ok) {
+            if (lane == 0) fail(kDenseErrMmaStage);
             break;
           }
           tc_fence_after();
-          const uint32_t a = smem_u32(base + s * C::STAGE_BYTES), b = a + C::A_BYTES;
+          const uint32_t a = base_u + s * C::STAGE_BYTES, b = a + C::A_BYTES;
           const uint64_t da = desc(a, A_MN), db = desc(b, B_MN);
-          if constexpr (C::F32) {
-            const uint32_t alo = b + C::B_BYTES, blo = alo + C::A_BYTES;
-            const uint64_t dal = desc(alo, A_MN), dbl = desc(blo, B_MN);
+          --left;
+          if (elect_one()) {
+            if constexpr (C::F32) {
+              const uint32_t alo = b + C::B_BYTES, blo = alo + C::A_BYTES;
+              const uint64_t dal = desc(alo, A_MN), dbl = desc(blo, B_MN);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t more = !fresh || k > 0;
-              mma(d, da + step_a * k, db + step_b * k, more);
-              mma(d + BN, da + step_a * k, dbl + step_b * k, more);
-              mma(d + BN, dal + step_a * k, db + step_b * k, 1u);
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t more = !fresh || k > 0;
+                mma(d, da + step_a * k, db + step_b * k, more);
+                mma(d + BN, da + step_a * k, dbl + step_b * k, more);
+                mma(d + BN, dal + step_a * k, db + step_b * k, 1u);
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma(d, da + step_a * k, db + step_b * k, !fresh || k > 0);
             }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma(d, da + step_a * k, db + step_b * k, !fresh || k > 0);
+            commit(&empty[s]);
+            if (left == 0) commit(&acc_full[tc & 1]);
           }
-          commit(&empty[s]);
-          if ((kb - k0) % C::CHUNK == C::CHUNK - 1 || kb == k1 - 1) commit(&acc_full[tc++ & 1]);
+          __syncwarp();
+          if (left == 0) ++tc;
+          if (++s == C::STAGES) s = 0, ph ^= 1;
         }
       }
-      if (*vabort) {
-        commit(drained);
+      if (!ok) {
+        if (elect_one()) commit(drained);
+        __syncwarp();
         wait(drained, 0);
       }
     }

@@ -78,6 +78,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const 
   }
 }
 
+// One lane of a converged warp, the same one each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+  return on != 0;
+}
+
 // ---------------------------------------------------------- CTA pairs
 // Two CTAs of a cluster that work on one tile (cta_group::2). A barrier of
 // the pair's leader is reached through its shared::cluster address.
