@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(256)
 //                quarter, each with half the columns
 //   warps 12-15  fp32 only: the TF32 split (as in the executor's kernels:
 //                the fp32 tile itself is hi, read truncated to TF32; these
-//                warps write lo = x - hi beside it)
+//                warps write lo = x - hi to a ring beside it)
 // Two accumulator sets let the epilogue of one tile overlap the products of
 // the next. In fp32 a set is two regions, hi*hi and the cross terms
 // hi*lo + lo*hi, and the epilogue takes a set every kChunk k-blocks and adds
@@ -315,8 +315,12 @@ struct DenseCfg {
   static constexpr int BROWS = BN / G;  // rows of B a CTA loads
   static constexpr int A_BYTES = 128 * 128;
   static constexpr int B_BYTES = BROWS * 128;
-  static constexpr int STAGE_BYTES = (A_BYTES + B_BYTES) * (F32 ? 2 : 1);
-  static constexpr int STAGES = (192 * 1024 / STAGE_BYTES) < 8 ? (192 * 1024 / STAGE_BYTES) : 8;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  // fp32: the lo halves have a shorter ring of their own, so that more of the
+  // shared memory holds loads in flight.
+  static constexpr int LO_STAGES = F32 ? 2 : 0;
+  static constexpr int FIT = 192 * 1024 / STAGE_BYTES - LO_STAGES;
+  static constexpr int STAGES = FIT < 8 ? FIT : 8;
   static constexpr int SET_COLS = F32 ? 2 * BN : BN;
   static constexpr int TMEM_COLS = 2 * SET_COLS;
   static constexpr int CHUNK = F32 ? 8 : 1 << 30;  // k-blocks a set accumulates
@@ -327,7 +331,7 @@ struct DenseCfg {
   // j ^ (r & 7), so that neither the writes (a lane a row) nor the reads (four
   // lanes a row) meet in a bank.
   static constexpr int STAGING_BYTES = EPI_WARPS * 4096;
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + STAGING_BYTES + 8 * (3 * STAGES + 5) + 16;
+  static constexpr int SMEM_BYTES = 1024 + (STAGES + LO_STAGES) * STAGE_BYTES + STAGING_BYTES + 8 * (2 * STAGES + 2 * LO_STAGES + 5) + 16;
   static_assert(SMEM_BYTES <= 232448 - 64, "shared memory per CTA");
   static_assert(TMEM_COLS <= 512, "TMEM columns");
 };
@@ -387,11 +391,13 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
   using namespace sm100;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* staging = reinterpret_cast<float*>(base + C::STAGES * C::STAGE_BYTES);
-  uint64_t* full = reinterpret_cast<uint64_t*>(base + C::STAGES * C::STAGE_BYTES + C::STAGING_BYTES);
+  uint8_t* lo_base = base + C::STAGES * C::STAGE_BYTES;
+  float* staging = reinterpret_cast<float*>(lo_base + C::LO_STAGES * C::STAGE_BYTES);
+  uint64_t* full = reinterpret_cast<uint64_t*>(lo_base + C::LO_STAGES * C::STAGE_BYTES + C::STAGING_BYTES);
   uint64_t* empty = full + C::STAGES;
   uint64_t* lo_ready = empty + C::STAGES;
-  uint64_t* acc_full = lo_ready + C::STAGES;
+  uint64_t* lo_empty = lo_ready + C::LO_STAGES;
+  uint64_t* acc_full = lo_empty + C::LO_STAGES;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* drained = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
@@ -408,7 +414,10 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
-      mbar_init(&lo_ready[s], G * (C::F32 ? C::SPLIT_WARPS : 1));
+    }
+    for (int s = 0; s < C::LO_STAGES; ++s) {
+      mbar_init(&lo_ready[s], G * C::SPLIT_WARPS);
+      mbar_init(&lo_empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
@@ -530,8 +539,8 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
             mma_f16(d, da, db, idesc, more);
         }
       };
-      const uint32_t base_u = smem_u32(base);
-      uint32_t s = 0, ph = 0, tc = 0;
+      const uint32_t base_u = smem_u32(base), lo_u = smem_u32(lo_base);
+      uint32_t s = 0, ph = 0, l = 0, lph = 0, tc = 0;
       bool ok = true;
       for (int w = first; w < items && ok; w += step) {
         int k0, k1;
@@ -550,7 +559,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
             d = tmem + acc * C::SET_COLS;
             left = min(C::CHUNK, k1 - kb);
           }
-          ok = __all_sync(0xFFFFFFFFu, wait(C::F32 ? &lo_ready[s] : &full[s], ph));
+          ok = __all_sync(0xFFFFFFFFu, C::F32 ? wait(&lo_ready[l], lph) : wait(&full[s], ph));
           if (!ok) {
             if (lane == 0) fail(kDenseErrMmaStage);
             break;
@@ -561,7 +570,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
           --left;
           if (elect_one()) {
             if constexpr (C::F32) {
-              const uint32_t alo = b + C::B_BYTES, blo = alo + C::A_BYTES;
+              const uint32_t alo = lo_u + l * C::STAGE_BYTES, blo = alo + C::A_BYTES;
               const uint64_t dal = desc(alo, A_MN), dbl = desc(blo, B_MN);
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
@@ -575,11 +584,13 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
               for (int k = 0; k < 4; ++k) mma(d, da + step_a * k, db + step_b * k, !fresh || k > 0);
             }
             commit(&empty[s]);
+            if constexpr (C::F32) commit(&lo_empty[l]);
             if (left == 0) commit(&acc_full[tc & 1]);
           }
           __syncwarp();
           if (left == 0) ++tc;
           if (++s == C::STAGES) s = 0, ph ^= 1;
+          if (C::F32 && ++l == C::LO_STAGES) l = 0, lph ^= 1;
         }
       }
       if (!ok) {
@@ -647,31 +658,36 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
         }
       }
     }
-  } else if (C::F32 && warp >= C::SPLIT_WARP0) {
+  }
+  if constexpr (C::F32) if (warp >= C::SPLIT_WARP0) {
     const int tid = threadIdx.x - 32 * C::SPLIT_WARP0;
-    uint32_t it = 0;
+    uint32_t s = 0, ph = 0, l = 0, lph = 0;
     bool ok = true;
     for (int w = first; w < items && ok; w += step) {
       int k0, k1;
       kb_range(w / tiles, k0, k1);
-      for (int kb = k0; kb < k1; ++kb, ++it) {
-        const int s = it % C::STAGES;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&full[s], (it / C::STAGES) & 1, vabort));
+      for (int kb = k0; kb < k1; ++kb) {
+        ok = __all_sync(0xFFFFFFFFu, wait(&full[s], ph) && wait(&lo_empty[l], lph ^ 1));
         if (!ok) {
           if (lane == 0) fail(kDenseErrSplit);
           break;
         }
         // Elementwise, so the swizzled layouts do not matter.
         const float4* src = reinterpret_cast<const float4*>(base + s * C::STAGE_BYTES) + tid;
-        float4* dst = reinterpret_cast<float4*>(base + s * C::STAGE_BYTES + C::A_BYTES + C::B_BYTES) + tid;
-#pragma unroll 8
-        for (int i = 0; i < (C::A_BYTES + C::B_BYTES) / 16; i += 32 * C::SPLIT_WARPS) {
-          const float4 v = src[i];
-          dst[i] = make_float4(dense_residual(v.x), dense_residual(v.y), dense_residual(v.z), dense_residual(v.w));
-        }
+        float4* dst = reinterpret_cast<float4*>(lo_base + l * C::STAGE_BYTES) + tid;
+        constexpr int STEP = 32 * C::SPLIT_WARPS, PER = C::F32 ? C::STAGE_BYTES / 16 / STEP : 1;
+        float4 v[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] = src[i * STEP];
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          dst[i * STEP] = make_float4(dense_residual(v[i].x), dense_residual(v[i].y), dense_residual(v[i].z),
+                                      dense_residual(v[i].w));
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) arrive_leader(&lo_ready[s]);
+        if (lane == 0) arrive_leader(&lo_ready[l]);
+        if (++s == C::STAGES) s = 0, ph ^= 1;
+        if (++l == C::LO_STAGES) l = 0, lph ^= 1;
       }
     }
   }
