@@ -65,7 +65,7 @@ struct DenseEpi {
   int64_t residual_stride, y_stride, pre_stride;
   int act;
   float slope;
-  int vec_residual, vec_y, vec_pre;  // 16-byte aligned rows
+  int vec_residual, vec_y, vec_pre, vec_bias;  // 16-byte aligned rows
   float* part;                       // [splits][m][ldp] or null
   int64_t ldp;                       // a multiple of 8
 };
@@ -280,10 +280,9 @@ __global__ void __launch_bounds__(256)
 //   warp 0       TMA producer: 128 bytes of K (64 or 32 elements) a stage
 //   warp 1       MMA issuer (one lane, of the pair's leader)
 //   warp 2       TMEM owner
-//   warps 4-11   epilogue: TMEM -> registers -> shared memory (transposing, so
-//                that rows leave in 64-byte or longer runs) -> bias,
-//                activation, residual -> memory; two warps per TMEM lane
-//                quarter, each with half the columns
+//   warps 4-11   epilogue: TMEM -> registers -> bias, activation, residual ->
+//                shared memory -> TMA store; two warps per TMEM lane quarter,
+//                each with half the columns
 //   warps 12-15  fp32 only: the TF32 split (as in the executor's kernels:
 //                the fp32 tile itself is hi, read truncated to TF32; these
 //                warps write lo = x - hi to a ring beside it)
@@ -327,9 +326,7 @@ struct DenseCfg {
   static constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
   static constexpr int SPLIT_WARP0 = 12, SPLIT_WARPS = F32 ? 4 : 0;
   static constexpr int THREADS = 32 * (SPLIT_WARP0 + SPLIT_WARPS);
-  // Per epilogue warp 32 rows x 32 floats; 16-byte chunk j of row r lies at
-  // j ^ (r & 7), so that neither the writes (a lane a row) nor the reads (four
-  // lanes a row) meet in a bank.
+  // Per epilogue warp 32 rows x 32 floats.
   static constexpr int STAGING_BYTES = EPI_WARPS * 4096;
   static constexpr int SMEM_BYTES = 1024 + (STAGES + LO_STAGES) * STAGE_BYTES + STAGING_BYTES + 8 * (2 * STAGES + 2 * LO_STAGES + 5) + 16;
   static_assert(SMEM_BYTES <= 232448 - 64, "shared memory per CTA");
@@ -353,46 +350,126 @@ __device__ __forceinline__ float dense_residual(float v) {
   return __uint_as_float(__float_as_uint(__fsub_rn(v, hi)) + 0x1000u);
 }
 
-// A warp's 32 rows x 32 columns of sums, a row in each lane's v: through the
-// staging buffer into rows of 8 columns a lane, and out.
+// The epilogue of a warp's 32 rows x 32 columns of sums, a row in each lane:
+// bias, activation and residual there, 32 independent values a lane, then the
+// block is packed into the warp's 4 KB staging buffer in the swizzle of a
+// tensor map and leaves by TMA, which also clips it to the matrix. (The fp32
+// epilogue is bound by its few warps' instruction latency: with the block
+// read back and stored by the lanes, 71680 x 128 -> 256 fp32 with GELU and pre
+// took 58-70 us, EPINEW us this way.) Matrices that a tensor map cannot take
+// (unaligned rows) are written by the lanes, a column a lane.
 template <class T>
-__device__ __forceinline__ void dense_store32(const DenseMm& p, float4* st, const float* v, int lane, int split,
-                                              int64_t row0, int64_t col0) {
-  __syncwarp();  // the buffer's last reads
+struct DenseOut {
+  static constexpr int V = kVec<T>;
+  const DenseMm& p;
+  const CUtensorMap *ty, *tpre;
+  uint8_t* buf;
+  int lane;
+  int turn = 0;  // 16-bit blocks take half the buffer: the halves alternate
+
+  // Columns [col0, col0 + 32) of a vector or of this lane's row; zero past n.
+  __device__ __forceinline__ void row32(const T* q, bool vec, int64_t col0, float* v) const {
+    if (vec && col0 + 32 <= p.n) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 4)
-    st[lane * 8 + ((i / 4) ^ (lane & 7))] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-  __syncwarp();
-  const int64_t col = col0 + (lane & 3) * 8;
-  const int valid = int(p.n - col < 8 ? p.n - col : 8);
-  float bias[8];
-  if (!p.epi.part) load_bias<T>(p.epi, col, valid, bias);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2);
-    const int64_t row = row0 + r;
-    const float4 lo = st[r * 8 + ((2 * (lane & 3)) ^ (r & 7))];
-    const float4 hi = st[r * 8 + ((2 * (lane & 3) + 1) ^ (r & 7))];
-    if (row >= p.m || valid <= 0) continue;
-    if (p.epi.part) {
-      float4* o = reinterpret_cast<float4*>(p.epi.part + (int64_t(split) * p.m + row) * p.epi.ldp + col);
-      o[0] = lo, o[1] = hi;
+      for (int i = 0; i < 32; i += V) raw_unpack<T, V>(raw_load<T, V>(q + col0 + i), v + i);
     } else {
-      float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-      dense_finish<T>(p.epi, x, bias, row, col, valid);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = col0 + i < p.n ? to_f(q[col0 + i]) : 0.0f;
     }
   }
-}
+  __device__ __forceinline__ void bias(int64_t col0, float* v) const {
+    if (p.epi.part || !p.epi.bias) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+    } else {
+      row32(static_cast<const T*>(p.epi.bias), p.epi.vec_bias, col0, v);
+    }
+  }
+  // The block into the buffer as U: rows of 128 bytes (64 with 2-byte
+  // elements), 16-byte chunk j of row r at j ^ (r % 8) (j ^ (r / 2 % 4)), which
+  // is the tensor maps' 128-byte (64-byte) swizzle and free of bank conflicts.
+  template <class U>
+  __device__ __forceinline__ uint8_t* stage(const float* v) {
+    constexpr int W = kVec<U>, CH = 32 / W;
+    constexpr bool HALF = sizeof(U) == 2;
+    if (lane == 0) {
+      if (HALF)
+        sm100::bulk_wait_read<1>();
+      else
+        sm100::bulk_wait_read<0>();
+    }
+    __syncwarp();
+    uint8_t* at = buf + (HALF ? (turn & 1) * 2048 : 0);
+    turn += HALF;
+    const int x = HALF ? (lane >> 1) & 3 : lane & 7;
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+      *reinterpret_cast<uint4*>(at + lane * CH * 16 + ((j ^ x) << 4)) = raw_pack<U, W>(v + j * W).u;
+    return at;
+  }
+  template <class U>
+  __device__ __forceinline__ void emit(const CUtensorMap* map, const float* v, int64_t row0, int64_t col0, int z) {
+    uint8_t* at = stage<U>(v);
+    sm100::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      sm100::tma_store_3d(map, at, int(col0), int(row0), z);
+      sm100::bulk_commit();
+    }
+  }
+  __device__ __forceinline__ void put(T* out, int64_t stride, bool vec, const CUtensorMap* map, const float* v,
+                                      int64_t row0, int64_t col0) {
+    if (vec) return emit<T>(map, v, row0, col0, 0);
+    const float* st = reinterpret_cast<const float*>(stage<float>(v));
+    __syncwarp();
+    if (col0 + lane < p.n) {
+      T* o = out + row0 * stride + col0 + lane;
+      const int rows = int(p.m - row0 < 32 ? p.m - row0 : 32);
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r) o[r * stride] = from_f<T>(st[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)]);
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ void finish(float* v, int split, int64_t row0, int64_t col0) {
+    const DenseEpi& e = p.epi;
+    if (row0 >= p.m || col0 >= p.n) return;
+    if (e.part) return emit<float>(ty, v, row0, col0, split);
+    float res[32];
+    if (e.residual && row0 + lane < p.m)
+      row32(static_cast<const T*>(e.residual) + (row0 + lane) * e.residual_stride, e.vec_residual, col0, res);
+    if (e.pre) put(static_cast<T*>(e.pre), e.pre_stride, e.vec_pre, tpre, v, row0, col0);
+    if (e.act == MX_ACT_GELU) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) gelu_f2(v[i], v[i + 1]);
+    } else if (e.act == MX_ACT_LRELU) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = v[i] >= 0.0f ? v[i] : e.slope * v[i];
+    } else if (e.act == MX_ACT_SIGMOID) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = sigmoid_f(v[i]);
+    }
+    if (e.residual && row0 + lane < p.m) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] += res[i];
+    }
+    put(static_cast<T*>(e.y), e.y_stride, e.vec_y, ty, v, row0, col0);
+  }
+  __device__ __forceinline__ void done() const {
+    if (lane == 0) sm100::bulk_wait<0>();
+    __syncwarp();
+  }
+};
 
 template <class T, bool A_MN, bool B_MN, int BN, int G>
 __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
-    dense_mm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, DenseMm p) {
+    dense_mm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmPre, DenseMm p) {
   using C = DenseCfg<T, BN, G>;
   using namespace sm100;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* lo_base = base + C::STAGES * C::STAGE_BYTES;
-  float* staging = reinterpret_cast<float*>(lo_base + C::LO_STAGES * C::STAGE_BYTES);
+  uint8_t* staging = lo_base + C::LO_STAGES * C::STAGE_BYTES;
   uint64_t* full = reinterpret_cast<uint64_t*>(lo_base + C::LO_STAGES * C::STAGE_BYTES + C::STAGING_BYTES);
   uint64_t* empty = full + C::STAGES;
   uint64_t* lo_ready = empty + C::STAGES;
@@ -601,7 +678,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
     }
   } else if (warp >= C::EPI_WARP0 && warp < C::EPI_WARP0 + C::EPI_WARPS) {
     const int ew = warp - C::EPI_WARP0, q = warp & 3, half = ew >> 2;
-    float4* st = reinterpret_cast<float4*>(staging + ew * 1024);
+    DenseOut<T> out{p, &tmY, &tmPre, staging + ew * 4096, lane};
     uint32_t tc = 0;
     bool ok = true;
     for (int w = first; w < items && ok; w += step) {
@@ -628,7 +705,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
         constexpr int COLS = BN / 2;
         float sum[COLS];
 #pragma unroll
-        for (int i = 0; i < COLS; ++i) sum[i] = 0.0f;
+        for (int c = 0; c < COLS; c += 32) out.bias(col0 + c, sum + c);
         for (int kb = k0; kb < k1 && ok; kb += C::CHUNK) {
           ok = take();
           if (!ok) break;
@@ -644,20 +721,24 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
         }
         if (!ok) break;
 #pragma unroll
-        for (int c = 0; c < COLS; c += 32) dense_store32<T>(p, st, sum + c, lane, split, row0, col0 + c);
+        for (int c = 0; c < COLS; c += 32) out.finish(sum + c, split, row0, col0 + c);
       } else {
         ok = take();
         if (!ok) break;
         const uint32_t d = tmem + (uint32_t(q * 32) << 16) + (tc & 1) * C::SET_COLS + half * (BN / 2);
 #pragma unroll 1
         for (int c = 0; c < BN / 2; c += 32) {
-          float v[32];
+          float v[32], b[32];
+          out.bias(col0 + c, b);
           tmem_ld32(d + c, v);
           if (c + 32 == BN / 2) give();
-          dense_store32<T>(p, st, v, lane, split, row0, col0 + c);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += b[i];
+          out.finish(v, split, row0, col0 + c);
         }
       }
     }
+    out.done();
   }
   if constexpr (C::F32) if (warp >= C::SPLIT_WARP0) {
     const int tid = threadIdx.x - 32 * C::SPLIT_WARP0;

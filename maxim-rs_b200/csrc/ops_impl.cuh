@@ -241,23 +241,41 @@ MmPlan plan_mm(int64_t m, int64_t n, int64_t k, int sms) {
 }
 
 template <class T>
+constexpr CUtensorMapDataType map_type() {
+  return sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                        : (std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+}
+
+template <class T>
 CUtensorMap operand_map(const Operand& o, int64_t rows, int64_t cols, int box_rows) {
   constexpr int BK = 128 / int(sizeof(T));
   const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
   const cuuint64_t strides[1] = {cuuint64_t(o.stride) * sizeof(T)};
   const cuuint32_t box[2] = {cuuint32_t(BK), cuuint32_t(box_rows)};
   const cuuint32_t es[2] = {1, 1};
-  const CUtensorMapDataType dt = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                 : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   // The swizzle the tensor core expects of the tile: 32-bit MN-major operands
   // have a form of their own.
   const CUtensorMapSwizzle sw =
       o.mn_major && sizeof(T) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B;
   CUtensorMap m;
-  CUresult r = tensor_map_encoder()(&m, dt, 2, const_cast<void*>(o.p), dims, strides, box, es,
+  CUresult r = tensor_map_encoder()(&m, map_type<T>(), 2, const_cast<void*>(o.p), dims, strides, box, es,
                                     CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw Error(fmt("cuTensorMapEncodeTiled failed (%d)", int(r)), MX_E_CUDA);
+  return m;
+}
+
+// A result's map: blocks of 32 x 32, in the swizzle the epilogue stages them in.
+template <class U>
+CUtensorMap result_map(void* p, int64_t stride, int64_t rows, int64_t cols, int64_t layers) {
+  const cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(layers)};
+  const cuuint64_t strides[2] = {cuuint64_t(stride) * sizeof(U), cuuint64_t(stride) * sizeof(U) * cuuint64_t(rows)};
+  const cuuint32_t box[3] = {32, 32, 1}, es[3] = {1, 1, 1};
+  CUtensorMap m;
+  CUresult r = tensor_map_encoder()(&m, map_type<U>(), 3, p, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                    sizeof(U) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                                    CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw Error(fmt("cuTensorMapEncodeTiled failed (%d)", int(r)), MX_E_CUDA);
   return m;
 }
@@ -280,6 +298,11 @@ void launch_mm(const Operand& a, const Operand& b, const DenseMm& p, int64_t k, 
   }
   const CUtensorMap ta = A_MN ? operand_map<T>(a, k, p.m, C::BK) : operand_map<T>(a, p.m, k, 128);
   const CUtensorMap tb = B_MN ? operand_map<T>(b, k, p.n, C::BK) : operand_map<T>(b, p.n, k, C::BROWS);
+  // Results that no map can take have none (the kernel does not touch theirs).
+  const CUtensorMap ty = p.epi.part ? result_map<float>(p.epi.part, p.epi.ldp, p.m, p.n, p.splits)
+                         : p.epi.vec_y ? result_map<T>(p.epi.y, p.epi.y_stride, p.m, p.n, 1) : CUtensorMap{};
+  const CUtensorMap tpre =
+      !p.epi.part && p.epi.vec_pre ? result_map<T>(p.epi.pre, p.epi.pre_stride, p.m, p.n, 1) : CUtensorMap{};
   const int64_t items = int64_t(p.tiles_m) * p.tiles_n * p.splits;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(std::min<int64_t>(items, d.sms / G) * G));
@@ -291,7 +314,7 @@ void launch_mm(const Operand& a, const Operand& b, const DenseMm& p, int64_t k, 
   at[0].val.clusterDim.x = G, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = G == 2 ? 1 : 0;
-  MX_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, p));
+  MX_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, ty, tpre, p));
 }
 
 // D = A B^T with the epilogue `epi`: the product, and the join of its splits.
@@ -422,6 +445,7 @@ void dense(const mx_dense_args& a, const OpsDevice& d, cudaStream_t s) {
   e.vec_residual = a.residual && aligned<T>(a.residual, a.residual_stride);
   e.vec_y = aligned<T>(a.y, a.y_stride);
   e.vec_pre = a.pre && aligned<T>(a.pre, a.pre_stride);
+  e.vec_bias = a.bias && aligned<T>(a.bias, 0);
   if (a.m <= kRowsMax) return dense_rows<T>(a, e, d, s);
   Carver c{static_cast<uint8_t*>(a.workspace)};
   Staged<T> x(c, a.x, a.x_stride, a.m, a.k), w(c, a.w, a.w_stride, a.n, a.k);
