@@ -280,10 +280,10 @@ __global__ void __launch_bounds__(256)
 //   warp 0       TMA producer: 128 bytes of K (64 or 32 elements) a stage
 //   warp 1       MMA issuer (one lane, of the pair's leader)
 //   warp 2       TMEM owner
-//   warps 4-11   epilogue: TMEM -> registers -> bias, activation, residual ->
-//                shared memory -> TMA store; two warps per TMEM lane quarter,
-//                each with half the columns
-//   warps 12-15  fp32 only: the TF32 split (as in the executor's kernels:
+//   warps 4-19   epilogue: TMEM -> registers -> bias, activation, residual ->
+//   (or 4-11)    shared memory -> TMA store; four (two) warps per TMEM lane
+//                quarter share the tile's columns
+//   then four    fp32 only: the TF32 split (as in the executor's kernels:
 //                the fp32 tile itself is hi, read truncated to TF32; these
 //                warps write lo = x - hi to a ring beside it)
 // Two accumulator sets let the epilogue of one tile overlap the products of
@@ -323,11 +323,11 @@ struct DenseCfg {
   static constexpr int SET_COLS = F32 ? 2 * BN : BN;
   static constexpr int TMEM_COLS = 2 * SET_COLS;
   static constexpr int CHUNK = F32 ? 8 : 1 << 30;  // k-blocks a set accumulates
-  static constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
-  static constexpr int SPLIT_WARP0 = 12, SPLIT_WARPS = F32 ? 4 : 0;
+  static constexpr int EPI_WARP0 = 4, EPI_WARPS = BN >= 128 ? 16 : 8;
+  static constexpr int EPI_COLS = BN / (EPI_WARPS / 4);  // columns of a tile per epilogue warp
+  static constexpr int SPLIT_WARP0 = EPI_WARP0 + EPI_WARPS, SPLIT_WARPS = F32 ? 4 : 0;
   static constexpr int THREADS = 32 * (SPLIT_WARP0 + SPLIT_WARPS);
-  // Per epilogue warp 32 rows x 32 floats.
-  static constexpr int STAGING_BYTES = EPI_WARPS * 4096;
+  static constexpr int STAGING_BYTES = EPI_WARPS * 2048;  // 32 rows x 64 bytes each
   static constexpr int SMEM_BYTES = 1024 + (STAGES + LO_STAGES) * STAGE_BYTES + STAGING_BYTES + 8 * (2 * STAGES + 2 * LO_STAGES + 5) + 16;
   static_assert(SMEM_BYTES <= 232448 - 64, "shared memory per CTA");
   static_assert(TMEM_COLS <= 512, "TMEM columns");
@@ -352,12 +352,13 @@ __device__ __forceinline__ float dense_residual(float v) {
 
 // The epilogue of a warp's 32 rows x 32 columns of sums, a row in each lane:
 // bias, activation and residual there, 32 independent values a lane, then the
-// block is packed into the warp's 4 KB staging buffer in the swizzle of a
-// tensor map and leaves by TMA, which also clips it to the matrix. (The fp32
-// epilogue is bound by its few warps' instruction latency: with the block
-// read back and stored by the lanes, 71680 x 128 -> 256 fp32 with GELU and pre
-// took 58-70 us, EPINEW us this way.) Matrices that a tensor map cannot take
-// (unaligned rows) are written by the lanes, a column a lane.
+// block is packed into the warp's 2 KB staging buffer in the swizzle of a
+// tensor map and leaves by TMA, which also clips it to the matrix. (Where K is
+// short the epilogue sets the pace, by its warps' instruction latency: 71680 x
+// 128 -> 256 fp32 with GELU and pre took 58-70 us with the block read back and
+// stored by the lanes of 8 warps, 48 with TMA, EPINEW with 16 warps.) Matrices
+// that a tensor map cannot take (unaligned rows) are written by the lanes, a
+// column a lane.
 template <class T>
 struct DenseOut {
   static constexpr int V = kVec<T>;
@@ -365,7 +366,6 @@ struct DenseOut {
   const CUtensorMap *ty, *tpre;
   uint8_t* buf;
   int lane;
-  int turn = 0;  // 16-bit blocks take half the buffer: the halves alternate
 
   // Columns [col0, col0 + 32) of a vector or of this lane's row; zero past n.
   __device__ __forceinline__ void row32(const T* q, bool vec, int64_t col0, float* v) const {
@@ -385,58 +385,56 @@ struct DenseOut {
       row32(static_cast<const T*>(p.epi.bias), p.epi.vec_bias, col0, v);
     }
   }
-  // The block into the buffer as U: rows of 128 bytes (64 with 2-byte
-  // elements), 16-byte chunk j of row r at j ^ (r % 8) (j ^ (r / 2 % 4)), which
-  // is the tensor maps' 128-byte (64-byte) swizzle and free of bank conflicts.
+  // 64 bytes a row of the block (32 columns, or 16 in fp32) into the buffer as U:
+  // 16-byte chunk j of row r at j ^ (r / 2 % 4), which is the tensor maps'
+  // 64-byte swizzle and free of bank conflicts.
   template <class U>
-  __device__ __forceinline__ uint8_t* stage(const float* v) {
-    constexpr int W = kVec<U>, CH = 32 / W;
-    constexpr bool HALF = sizeof(U) == 2;
-    if (lane == 0) {
-      if (HALF)
-        sm100::bulk_wait_read<1>();
-      else
-        sm100::bulk_wait_read<0>();
-    }
+  __device__ __forceinline__ void stage(const float* v) {
+    constexpr int W = kVec<U>;
+    if (lane == 0) sm100::bulk_wait_read<0>();
     __syncwarp();
-    uint8_t* at = buf + (HALF ? (turn & 1) * 2048 : 0);
-    turn += HALF;
-    const int x = HALF ? (lane >> 1) & 3 : lane & 7;
 #pragma unroll
-    for (int j = 0; j < CH; ++j)
-      *reinterpret_cast<uint4*>(at + lane * CH * 16 + ((j ^ x) << 4)) = raw_pack<U, W>(v + j * W).u;
-    return at;
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = raw_pack<U, W>(v + j * W).u;
   }
   template <class U>
   __device__ __forceinline__ void emit(const CUtensorMap* map, const float* v, int64_t row0, int64_t col0, int z) {
-    uint8_t* at = stage<U>(v);
-    sm100::fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      sm100::tma_store_3d(map, at, int(col0), int(row0), z);
-      sm100::bulk_commit();
+    constexpr int COLS = 64 / int(sizeof(U));
+#pragma unroll
+    for (int h = 0; h < 32; h += COLS) {
+      if (h > 0 && col0 + h >= p.n) break;
+      stage<U>(v + h);
+      sm100::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        sm100::tma_store_3d(map, buf, int(col0) + h, int(row0), z);
+        sm100::bulk_commit();
+      }
     }
   }
   __device__ __forceinline__ void put(T* out, int64_t stride, bool vec, const CUtensorMap* map, const float* v,
                                       int64_t row0, int64_t col0) {
     if (vec) return emit<T>(map, v, row0, col0, 0);
-    const float* st = reinterpret_cast<const float*>(stage<float>(v));
-    __syncwarp();
-    if (col0 + lane < p.n) {
-      T* o = out + row0 * stride + col0 + lane;
-      const int rows = int(p.m - row0 < 32 ? p.m - row0 : 32);
+    const int c = lane & 15;
+    const int rows = int(p.m - row0 < 32 ? p.m - row0 : 32);
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      stage<float>(v + h);
+      __syncwarp();
+      if (col0 + h + c < p.n) {
+        T* o = out + row0 * stride + col0 + h + c;
 #pragma unroll 8
-      for (int r = 0; r < rows; ++r) o[r * stride] = from_f<T>(st[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)]);
+        for (int r = lane >> 4; r < rows; r += 2)
+          o[r * stride] = from_f<T>(
+              *reinterpret_cast<const float*>(buf + r * 64 + (((c >> 2) ^ ((r >> 1) & 3)) << 4) + (c & 3) * 4));
+      }
+      __syncwarp();
     }
-    __syncwarp();
   }
   __device__ __forceinline__ void finish(float* v, int split, int64_t row0, int64_t col0) {
     const DenseEpi& e = p.epi;
     if (row0 >= p.m || col0 >= p.n) return;
     if (e.part) return emit<float>(ty, v, row0, col0, split);
-    float res[32];
-    if (e.residual && row0 + lane < p.m)
-      row32(static_cast<const T*>(e.residual) + (row0 + lane) * e.residual_stride, e.vec_residual, col0, res);
     if (e.pre) put(static_cast<T*>(e.pre), e.pre_stride, e.vec_pre, tpre, v, row0, col0);
     if (e.act == MX_ACT_GELU) {
 #pragma unroll
@@ -449,8 +447,10 @@ struct DenseOut {
       for (int i = 0; i < 32; ++i) v[i] = sigmoid_f(v[i]);
     }
     if (e.residual && row0 + lane < p.m) {
+      float r[32];
+      row32(static_cast<const T*>(e.residual) + (row0 + lane) * e.residual_stride, e.vec_residual, col0, r);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] += res[i];
+      for (int i = 0; i < 32; ++i) v[i] += r[i];
     }
     put(static_cast<T*>(e.y), e.y_stride, e.vec_y, ty, v, row0, col0);
   }
@@ -677,8 +677,8 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
       }
     }
   } else if (warp >= C::EPI_WARP0 && warp < C::EPI_WARP0 + C::EPI_WARPS) {
-    const int ew = warp - C::EPI_WARP0, q = warp & 3, half = ew >> 2;
-    DenseOut<T> out{p, &tmY, &tmPre, staging + ew * 4096, lane};
+    const int ew = warp - C::EPI_WARP0, q = warp & 3, part = ew >> 2;
+    DenseOut<T> out{p, &tmY, &tmPre, staging + ew * 2048, lane};
     uint32_t tc = 0;
     bool ok = true;
     for (int w = first; w < items && ok; w += step) {
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
       const int split = w / tiles;
       kb_range(split, k0, k1);
       const int64_t row0 = (int64_t(tm) * G + rank) * 128 + q * 32;
-      const int64_t col0 = int64_t(tn) * BN + half * (BN / 2);
+      const int64_t col0 = int64_t(tn) * BN + part * C::EPI_COLS;
       // The warp decides as one: the TMEM loads below need all its lanes.
       auto take = [&] {
         const bool got = __all_sync(0xFFFFFFFFu, wait(&acc_full[tc & 1], (tc >> 1) & 1));
@@ -702,16 +702,15 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
         ++tc;
       };
       if constexpr (C::F32) {
-        constexpr int COLS = BN / 2;
-        float sum[COLS];
-#pragma unroll
-        for (int c = 0; c < COLS; c += 32) out.bias(col0 + c, sum + c);
+        static_assert(!C::F32 || C::EPI_COLS == 32, "one block a warp");
+        float sum[32];
+        out.bias(col0, sum);
         for (int kb = k0; kb < k1 && ok; kb += C::CHUNK) {
           ok = take();
           if (!ok) break;
-          const uint32_t d = tmem + (uint32_t(q * 32) << 16) + (tc & 1) * C::SET_COLS + half * COLS;
+          const uint32_t d = tmem + (uint32_t(q * 32) << 16) + (tc & 1) * C::SET_COLS + part * 32;
 #pragma unroll
-          for (int c = 0; c < COLS; c += 16) {
+          for (int c = 0; c < 32; c += 16) {
             float hh[16], cross[16];
             tmem_ld16x2(d + c, d + BN + c, hh, cross);
 #pragma unroll
@@ -720,18 +719,17 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
           give();
         }
         if (!ok) break;
-#pragma unroll
-        for (int c = 0; c < COLS; c += 32) out.finish(sum + c, split, row0, col0 + c);
+        out.finish(sum, split, row0, col0);
       } else {
         ok = take();
         if (!ok) break;
-        const uint32_t d = tmem + (uint32_t(q * 32) << 16) + (tc & 1) * C::SET_COLS + half * (BN / 2);
+        const uint32_t d = tmem + (uint32_t(q * 32) << 16) + (tc & 1) * C::SET_COLS + part * C::EPI_COLS;
 #pragma unroll 1
-        for (int c = 0; c < BN / 2; c += 32) {
+        for (int c = 0; c < C::EPI_COLS; c += 32) {
           float v[32], b[32];
           out.bias(col0 + c, b);
           tmem_ld32(d + c, v);
-          if (c + 32 == BN / 2) give();
+          if (c + 32 == C::EPI_COLS) give();
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] += b[i];
           out.finish(v, split, row0, col0 + c);

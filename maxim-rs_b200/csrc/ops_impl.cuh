@@ -266,16 +266,15 @@ CUtensorMap operand_map(const Operand& o, int64_t rows, int64_t cols, int box_ro
   return m;
 }
 
-// A result's map: blocks of 32 x 32, in the swizzle the epilogue stages them in.
+// A result's map: blocks of 32 rows x 64 bytes, in the swizzle the epilogue stages them in.
 template <class U>
 CUtensorMap result_map(void* p, int64_t stride, int64_t rows, int64_t cols, int64_t layers) {
   const cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(layers)};
   const cuuint64_t strides[2] = {cuuint64_t(stride) * sizeof(U), cuuint64_t(stride) * sizeof(U) * cuuint64_t(rows)};
-  const cuuint32_t box[3] = {32, 32, 1}, es[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64 / sizeof(U), 32, 1}, es[3] = {1, 1, 1};
   CUtensorMap m;
   CUresult r = tensor_map_encoder()(&m, map_type<U>(), 3, p, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                    sizeof(U) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                                    CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                    CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw Error(fmt("cuTensorMapEncodeTiled failed (%d)", int(r)), MX_E_CUDA);
   return m;
 }
