@@ -141,7 +141,8 @@ __device__ __forceinline__ void f2_add_to(float& a, float& c, float b, float d) 
 // partial sum of Horner over u - the same magnitudes, rounded the same way -
 // and ends on exactly R(u); w e is then exactly -(u e), the scalar form's
 // first factor.
-__device__ __forceinline__ void gelu_f2(float& a, float& b) {
+// R(u) of two values given as -u.
+__device__ __forceinline__ uint64_t gelu_r2(uint64_t w) {
   constexpr float kGeluRw[12] = {
       0.4999999701976776f,
       0.3989405930042267f,
@@ -155,10 +156,14 @@ __device__ __forceinline__ void gelu_f2(float& a, float& b) {
       8.47700794111006e-05f,
       7.708666089456528e-06f,
       3.155372496621567e-07f};
-  const uint64_t w = f2_pack(fmaxf(-fabsf(a), -5.6f), fmaxf(-fabsf(b), -5.6f));
   uint64_t p = f2_pack(kGeluRw[11], kGeluRw[11]);
 #pragma unroll
   for (int k = 10; k >= 0; --k) p = f2_fma(p, w, f2_pack(kGeluRw[k], kGeluRw[k]));
+  return p;
+}
+__device__ __forceinline__ void gelu_f2(float& a, float& b) {
+  const uint64_t w = f2_pack(fmaxf(-fabsf(a), -5.6f), fmaxf(-fabsf(b), -5.6f));
+  const uint64_t p = gelu_r2(w);
   const uint64_t x = f2_pack(a, b);
   float ta, tb;
   f2_unpack(f2_mul(f2_mul(x, f2_pack(-0.72134752f, -0.72134752f)), x), ta, tb);

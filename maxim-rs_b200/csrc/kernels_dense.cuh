@@ -41,15 +41,42 @@ __device__ __forceinline__ float gelu_grad_f(float x) {
   const float phi = x < 0.0f ? t : 1.0f - t;
   return fmaf(fminf(fmaxf(x, -30.0f), 30.0f) * e, 0.3989422804f, phi);
 }
-__device__ __forceinline__ float act_grad(int act, float v, float slope) {
-  switch (act) {
-    case MX_ACT_GELU: return gelu_grad_f(v);
-    case MX_ACT_LRELU: return v >= 0.0f ? 1.0f : slope;
-    case MX_ACT_SIGMOID: {
-      const float s = sigmoid_f(v);
-      return s * (1.0f - s);
+// Two at once, by f32x2 instructions.
+__device__ __forceinline__ void gelu_grad_f2(float a, float b, float& ga, float& gb) {
+  const uint64_t x = f2_pack(a, b);
+  const uint64_t p = gelu_r2(f2_pack(fmaxf(-fabsf(a), -5.6f), fmaxf(-fabsf(b), -5.6f)));
+  float ta, tb, u, v;
+  f2_unpack(f2_mul(f2_mul(x, f2_pack(-0.72134752f, -0.72134752f)), x), ta, tb);
+  const uint64_t e = f2_pack(ex2_approx(ta), ex2_approx(tb));
+  f2_unpack(f2_mul(e, p), u, v);  // Phi(-|x|)
+  const uint64_t phi = f2_pack(a < 0.0f ? u : 1.0f - u, b < 0.0f ? v : 1.0f - v);
+  const uint64_t xc = f2_pack(fminf(fmaxf(a, -30.0f), 30.0f), fminf(fmaxf(b, -30.0f), 30.0f));
+  f2_unpack(f2_fma(f2_mul(xc, e), f2_pack(0.3989422804f, 0.3989422804f), phi), ga, gb);
+}
+// v[i] *= act'(q[i]).
+template <int N>
+__device__ __forceinline__ void apply_act_grad(int act, float* v, const float* q, float slope) {
+  if (act == MX_ACT_GELU) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        float a, b;
+        gelu_grad_f2(q[i], q[i + 1], a, b);
+        v[i] *= a, v[i + 1] *= b;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] *= gelu_grad_f(q[i]);
     }
-    default: return 1.0f;
+  } else if (act == MX_ACT_LRELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= q[i] >= 0.0f ? 1.0f : slope;
+  } else if (act == MX_ACT_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float s = sigmoid_f(q[i]);
+      v[i] *= s * (1.0f - s);
+    }
   }
 }
 
@@ -121,24 +148,46 @@ __device__ __forceinline__ void load_bias(const DenseEpi& e, int64_t col, int va
   for (int i = 0; i < 8; ++i) b[i] = e.bias && i < valid ? to_f(static_cast<const T*>(e.bias)[col + i]) : 0.0f;
 }
 
-// Sum of the partial products, in the order of the splits, and the epilogue.
-// One thread per 8 columns of a row.
-template <class T>
+// Sum of the partial products and the epilogue: a thread per 8 columns of a
+// row and, where there are few of those and many splits, `GROUPS` threads that
+// each add every GROUPS-th split and meet in shared memory. The order of a sum
+// depends on the number of splits alone.
+template <class T, int GROUPS>
 __global__ void __launch_bounds__(256) dense_join_kernel(DenseEpi e, int splits, int64_t m, int64_t n) {
+  constexpr int PER = 256 / GROUPS;
+  __shared__ float sums[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? PER * 8 : 1];
   const int64_t cols8 = (n + 7) / 8;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < m * cols8; i += int64_t(gridDim.x) * 256) {
-    const int64_t row = i / cols8, col = (i % cols8) * 8;
+  const int own = threadIdx.x % PER, group = threadIdx.x / PER;
+  for (int64_t i0 = int64_t(blockIdx.x) * PER; i0 < m * cols8; i0 += int64_t(gridDim.x) * PER) {
+    const int64_t i = i0 + own, row = i / cols8, col = (i % cols8) * 8;
     const int valid = int(n - col < 8 ? n - col : 8);
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, b[8];
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-      const float4* p = reinterpret_cast<const float4*>(e.part + (int64_t(s) * m + row) * e.ldp + col);
-      const float4 a = p[0], c = p[1];
-      v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
-      v[4] += c.x, v[5] += c.y, v[6] += c.z, v[7] += c.w;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (i < m * cols8) {
+#pragma unroll 8
+      for (int s = group; s < splits; s += GROUPS) {
+        const float4* p = reinterpret_cast<const float4*>(e.part + (int64_t(s) * m + row) * e.ldp + col);
+        const float4 a = p[0], c = p[1];
+        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
+        v[4] += c.x, v[5] += c.y, v[6] += c.z, v[7] += c.w;
+      }
     }
-    load_bias<T>(e, col, valid, b);
-    dense_finish<T>(e, v, b, row, col, valid);
+    if constexpr (GROUPS > 1) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sums[group][k * PER + own] = v[k];
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int g = 1; g < GROUPS; ++g)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] += sums[g][k * PER + own];
+      }
+      __syncthreads();
+    }
+    if (group == 0 && i < m * cols8) {
+      float b[8];
+      load_bias<T>(e, col, valid, b);
+      dense_finish<T>(e, v, b, row, col, valid);
+    }
   }
 }
 
@@ -225,19 +274,31 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int k = 0; k < V; ++k) a[k] = 0.0f;
   if (col < n) {
-#pragma unroll 4
-    for (int64_t r = int64_t(blockIdx.y) * 8 + sub; r < m; r += int64_t(gridDim.y) * 8) {
-      float v[V];
-      raw_unpack<T, V>(raw_load<T, V>(dy + r * dy_stride + col), v);
-      if (act != MX_ACT_NONE) {
-        float q[V];
-        raw_unpack<T, V>(raw_load<T, V>(pre + r * pre_stride + col), q);
+    // AHEAD rows' loads are on their way before the first is worked on.
+    constexpr int AHEAD = 4;
+    const int64_t step = int64_t(gridDim.y) * 8;
+    for (int64_t r0 = int64_t(blockIdx.y) * 8 + sub; r0 < m; r0 += AHEAD * step) {
+      Raw<T, V> dr[AHEAD], pr[AHEAD];
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] *= act_grad(act, q[k], slope);
-        raw_store<T, V>(d + r * d_stride + col, raw_pack<T, V>(v));
+      for (int i = 0; i < AHEAD; ++i) {
+        const int64_t r = r0 + i * step;
+        dr[i] = r < m ? raw_load<T, V>(dy + r * dy_stride + col) : raw_zero<T, V>();
+        if (act != MX_ACT_NONE) pr[i] = r < m ? raw_load<T, V>(pre + r * pre_stride + col) : raw_zero<T, V>();
       }
 #pragma unroll
-      for (int k = 0; k < V; ++k) a[k] += v[k];
+      for (int i = 0; i < AHEAD; ++i) {
+        const int64_t r = r0 + i * step;
+        float v[V];
+        raw_unpack<T, V>(dr[i], v);
+        if (act != MX_ACT_NONE) {
+          float q[V];
+          raw_unpack<T, V>(pr[i], q);
+          apply_act_grad<V>(act, v, q, slope);
+          if (r < m) raw_store<T, V>(d + r * d_stride + col, raw_pack<T, V>(v));
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) a[k] += v[k];
+      }
     }
   }
   if (!part) return;

@@ -344,8 +344,12 @@ void run_mm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64_t k,
     by_width(std::false_type(), std::false_type());
   if (plan.splits > 1) {
     const int64_t vecs = m * ceil_div(n, 8);
-    dense_join_kernel<T>
-        <<<unsigned(std::min<int64_t>(ceil_div(vecs, 256), int64_t(d.sms) * 8)), 256, 0, s>>>(p.epi, plan.splits, m, n);
+    // Eight threads an output where that still leaves the GPU short of threads.
+    if (plan.splits >= 16 && vecs < int64_t(d.sms) * 512)
+      dense_join_kernel<T, 8><<<unsigned(ceil_div(vecs, 32)), 256, 0, s>>>(p.epi, plan.splits, m, n);
+    else
+      dense_join_kernel<T, 1>
+          <<<unsigned(std::min<int64_t>(ceil_div(vecs, 256), int64_t(d.sms) * 8)), 256, 0, s>>>(p.epi, plan.splits, m, n);
     check_launch("dense join");
   }
 }
