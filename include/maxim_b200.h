@@ -411,8 +411,8 @@ int mx_layer_norm_backward(const mx_layer_norm_backward_args* a, void* stream);
  * convolution's [c_out][c_in]), y [m][n]. act is MX_ACT_*: GELU in its erf
  * form, leaky ReLU with `slope`, the logistic sigmoid. fp32 products are
  * 3xTF32 splits (about 21 significant bits a product, summed in fp32); an
- * infinite fp32 operand gives NaN where it is used. Up to 8 rows run as plain
- * fp32 sums. y may be the residual itself (same stride). */
+ * infinite fp32 operand gives NaN where it is used. One or two rows (up to
+ * eight where w is small) run as plain fp32 sums. y may be the residual itself (same stride). */
 typedef struct mx_dense_args {
   const void* x;
   const void* w;

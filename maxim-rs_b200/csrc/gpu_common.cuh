@@ -135,14 +135,12 @@ __device__ __forceinline__ void f2_add_to(float& a, float& c, float b, float d) 
   f2_unpack(f2_add(f2_pack(a, c), f2_pack(b, d)), a, c);
 }
 
-// gelu_f on two values at once, bit-identical to gelu_f on each. With
-// w = -u = max(-|x|, -5.6) and kGeluRw[k] = (-1)^k kGeluR[k] (the magnitudes:
-// R's coefficients alternate in sign), Horner over w gives (-1)^k times every
-// partial sum of Horner over u - the same magnitudes, rounded the same way -
-// and ends on exactly R(u); w e is then exactly -(u e), the scalar form's
-// first factor.
-// R(u) of two values given as -u.
-__device__ __forceinline__ uint64_t gelu_r2(uint64_t w) {
+// R(u) of two values given as w = -u, u in [0, 5.6]. With
+// kGeluRw[k] = (-1)^k kGeluR[k] (the magnitudes: R's coefficients alternate in
+// sign), Horner over w gives (-1)^k times every partial sum of Horner over u -
+// the same magnitudes, rounded the same way - and ends on exactly R(u).
+// `slope` is added to the coefficient of w: R(u) + slope w.
+__device__ __forceinline__ uint64_t gelu_r2(uint64_t w, float slope = 0.0f) {
   constexpr float kGeluRw[12] = {
       0.4999999701976776f,
       0.3989405930042267f,
@@ -158,9 +156,15 @@ __device__ __forceinline__ uint64_t gelu_r2(uint64_t w) {
       3.155372496621567e-07f};
   uint64_t p = f2_pack(kGeluRw[11], kGeluRw[11]);
 #pragma unroll
-  for (int k = 10; k >= 0; --k) p = f2_fma(p, w, f2_pack(kGeluRw[k], kGeluRw[k]));
+  for (int k = 10; k >= 0; --k) {
+    const float c = k == 1 ? kGeluRw[1] + slope : kGeluRw[k];
+    p = f2_fma(p, w, f2_pack(c, c));
+  }
   return p;
 }
+// gelu_f on two values at once, bit-identical to gelu_f on each: with
+// w = -u = max(-|x|, -5.6), w e is exactly -(u e), the scalar form's first
+// factor.
 __device__ __forceinline__ void gelu_f2(float& a, float& b) {
   const uint64_t w = f2_pack(fmaxf(-fabsf(a), -5.6f), fmaxf(-fabsf(b), -5.6f));
   const uint64_t p = gelu_r2(w);

@@ -29,35 +29,26 @@ __device__ __forceinline__ float act_value(int act, float v, float slope) {
   }
 }
 
-// d/dx [x Phi(x)] = Phi(x) + x phi(x), with Phi(-u) = exp(-u^2 / 2) R(u) as in
-// gelu_f and phi(x) = exp(-x^2 / 2) / sqrt(2 pi): one exponential serves both.
-// x is clamped in the product x phi(x), which is 0 long before +-30 (an
-// infinite x would make it inf * 0).
-__device__ __forceinline__ float gelu_grad_f(float x) {
-  const float u = fminf(fabsf(x), 5.6f);
-  const float p = gelu_r(u);
-  const float e = ex2_approx(__fmul_rn(__fmul_rn(x, -0.72134752f), x));
-  const float t = e * p;  // Phi(-u)
-  const float phi = x < 0.0f ? t : 1.0f - t;
-  return fmaf(fminf(fmaxf(x, -30.0f), 30.0f) * e, 0.3989422804f, phi);
-}
-// Two at once, by f32x2 instructions.
+// d/dx [x Phi(x)] = Phi(x) + x phi(x). With u = |x|, Phi(-u) = exp(-u^2 / 2) R(u)
+// as in gelu_f and phi(x) = c exp(-u^2 / 2), c = 1 / sqrt(2 pi), both terms share
+// the exponential: with t = exp(-u^2 / 2) (R(u) - c u) the derivative is t for
+// x < 0 and 1 - t otherwise, and R(u) - c u is R's polynomial with another
+// linear coefficient. (u is clamped to 5.6 as for R; past it the exponential
+// leaves nothing, and an infinite x gives no inf * 0.) On two values at once.
 __device__ __forceinline__ void gelu_grad_f2(float a, float b, float& ga, float& gb) {
   const uint64_t x = f2_pack(a, b);
-  const uint64_t p = gelu_r2(f2_pack(fmaxf(-fabsf(a), -5.6f), fmaxf(-fabsf(b), -5.6f)));
-  float ta, tb, u, v;
+  const uint64_t q = gelu_r2(f2_pack(fmaxf(-fabsf(a), -5.6f), fmaxf(-fabsf(b), -5.6f)), 0.3989422804f);
+  float ta, tb;
   f2_unpack(f2_mul(f2_mul(x, f2_pack(-0.72134752f, -0.72134752f)), x), ta, tb);
-  const uint64_t e = f2_pack(ex2_approx(ta), ex2_approx(tb));
-  f2_unpack(f2_mul(e, p), u, v);  // Phi(-|x|)
-  const uint64_t phi = f2_pack(a < 0.0f ? u : 1.0f - u, b < 0.0f ? v : 1.0f - v);
-  const uint64_t xc = f2_pack(fminf(fmaxf(a, -30.0f), 30.0f), fminf(fmaxf(b, -30.0f), 30.0f));
-  f2_unpack(f2_fma(f2_mul(xc, e), f2_pack(0.3989422804f, 0.3989422804f), phi), ga, gb);
+  f2_unpack(f2_mul(f2_pack(ex2_approx(ta), ex2_approx(tb)), q), ta, tb);
+  ga = a < 0.0f ? ta : 1.0f - ta;
+  gb = b < 0.0f ? tb : 1.0f - tb;
 }
 // v[i] *= act'(q[i]).
 template <int N>
 __device__ __forceinline__ void apply_act_grad(int act, float* v, const float* q, float slope) {
   if (act == MX_ACT_GELU) {
-    if constexpr (N % 2 == 0) {
+    if constexpr (N > 1) {
 #pragma unroll
       for (int i = 0; i < N; i += 2) {
         float a, b;
@@ -65,8 +56,9 @@ __device__ __forceinline__ void apply_act_grad(int act, float* v, const float* q
         v[i] *= a, v[i + 1] *= b;
       }
     } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] *= gelu_grad_f(q[i]);
+      float g, unused;
+      gelu_grad_f2(q[0], 0.0f, g, unused);
+      v[0] *= g;
     }
   } else if (act == MX_ACT_LRELU) {
 #pragma unroll
@@ -204,7 +196,7 @@ __global__ void __launch_bounds__(256)
   __shared__ float red[8][R * CPW];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = warp % ks;
-  const int64_t col0 = (int64_t(blockIdx.x) * (8 / ks) + warp / ks) * CPW;
+  const int64_t col0 = (int64_t(blockIdx.x) * (blockDim.x / 32 / ks) + warp / ks) * CPW;
   float acc[R][CPW];
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -261,23 +253,26 @@ __global__ void __launch_bounds__(256)
 // ------------------------------------------ the pre-activation's gradient
 // d = dy act'(pre) and the partial column sums of d (over fp32 values, before
 // d is rounded to the operands' type for the two products). A block takes
-// 32 V columns of a range of rows, 8 rows at a time. With act none nothing is
-// written but the sums.
+// lx V columns (lx = 32, or fewer lanes where the matrix is narrow) of a range of
+// rows, 256 / lx rows at a time. With act none nothing is written but the sums.
+// GELU's derivative is about 17 instructions an element, which in 16 bits is as
+// long as the memory's time.
 template <class T, int V>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)
     dense_grad_kernel(const T* dy, int64_t dy_stride, const T* pre, int64_t pre_stride, T* d, int64_t d_stride,
-                      float* part, int64_t m, int n, int act, float slope) {
-  __shared__ float sums[8][32 * V];
-  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
-  const int col = (blockIdx.x * 32 + lane) * V;
+                      float* part, int64_t m, int n, int lx_log2, int act, float slope) {
+  __shared__ float sums[256 * V];
+  const int lx = 1 << lx_log2, subs = 256 >> lx_log2;
+  const int lane = threadIdx.x & (lx - 1), sub = threadIdx.x >> lx_log2;
+  const int col = (blockIdx.x * lx + lane) * V;
   float a[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) a[k] = 0.0f;
   if (col < n) {
     // AHEAD rows' loads are on their way before the first is worked on.
     constexpr int AHEAD = 4;
-    const int64_t step = int64_t(gridDim.y) * 8;
-    for (int64_t r0 = int64_t(blockIdx.y) * 8 + sub; r0 < m; r0 += AHEAD * step) {
+    const int64_t step = int64_t(gridDim.y) * subs;
+    for (int64_t r0 = int64_t(blockIdx.y) * subs + sub; r0 < m; r0 += AHEAD * step) {
       Raw<T, V> dr[AHEAD], pr[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
@@ -303,31 +298,44 @@ __global__ void __launch_bounds__(256)
   }
   if (!part) return;
 #pragma unroll
-  for (int k = 0; k < V; ++k) sums[sub][lane * V + k] = a[k];
+  for (int k = 0; k < V; ++k) sums[sub * lx * V + lane * V + k] = a[k];
   __syncthreads();
-  for (int i = threadIdx.x; i < 32 * V; i += 256) {
-    const int cc = blockIdx.x * 32 * V + i;
+  for (int i = threadIdx.x; i < lx * V; i += 256) {
+    const int cc = blockIdx.x * lx * V + i;
     if (cc >= n) continue;
     float t = 0.0f;
-#pragma unroll
-    for (int g = 0; g < 8; ++g) t += sums[g][i];
+#pragma unroll 8
+    for (int g = 0; g < subs; ++g) t += sums[g * lx * V + i];
     part[int64_t(blockIdx.y) * n + cc] = t;
   }
 }
 
-// A copy of a matrix whose rows are not 16-byte aligned into one whose rows
-// are (what the tensor maps need). One thread per 16 bytes of the copy.
+// Copies of matrices whose rows are not 16-byte aligned into ones whose rows
+// are (what the tensor maps need), all that a call needs in one launch. One
+// thread per 16 bytes of a copy; matrix i has the blocks from first[i] on.
+struct DenseAlign {
+  static constexpr int MAX = 3;
+  const void* src[MAX];
+  void* dst[MAX];
+  int64_t src_stride[MAX], dst_stride[MAX], rows[MAX], cols[MAX];
+  unsigned first[MAX + 1];
+  int count;
+};
 template <class T>
-__global__ void __launch_bounds__(256)
-    dense_align_kernel(const T* src, int64_t src_stride, T* dst, int64_t dst_stride, int64_t rows, int64_t cols) {
+__global__ void __launch_bounds__(256) dense_align_kernel(const __grid_constant__ DenseAlign a) {
   constexpr int V = kVec<T>;
-  const int64_t vecs = dst_stride / V;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < rows * vecs; i += int64_t(gridDim.x) * 256) {
+  int m = 0;
+  while (m + 1 < a.count && blockIdx.x >= a.first[m + 1]) ++m;
+  const T* src = static_cast<const T*>(a.src[m]);
+  T* dst = static_cast<T*>(a.dst[m]);
+  const int64_t vecs = a.dst_stride[m] / V, total = a.rows[m] * vecs;
+  const int64_t step = int64_t(a.first[m + 1] - a.first[m]) * 256;
+  for (int64_t i = int64_t(blockIdx.x - a.first[m]) * 256 + threadIdx.x; i < total; i += step) {
     const int64_t r = i / vecs, c = (i % vecs) * V;
     float v[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = c + k < cols ? to_f(src[r * src_stride + c + k]) : 0.0f;
-    raw_store<T, V>(dst + r * dst_stride + c, raw_pack<T, V>(v));
+    for (int k = 0; k < V; ++k) v[k] = c + k < a.cols[m] ? to_f(src[r * a.src_stride[m] + c + k]) : 0.0f;
+    raw_store<T, V>(dst + r * a.dst_stride[m] + c, raw_pack<T, V>(v));
   }
 }
 

@@ -207,7 +207,8 @@ struct MmPlan {
 // time, in one SM's cycles. A k-block (128 bytes of K) of a tile costs `step`
 // cycles, a tile's first loads and last epilogue about 3000; the CTAs of the
 // slowest SM are what counts. Split sums cost their write and reading back
-// (about 2000 bytes a cycle for the whole GPU) and another launch (about 4000).
+// (about 2000 bytes a cycle for the whole GPU) and another launch (about 6000, most of
+// it the host's).
 template <class T>
 MmPlan plan_mm(int64_t m, int64_t n, int64_t k, int sms) {
   constexpr bool F32 = sizeof(T) == 4;
@@ -230,7 +231,7 @@ MmPlan plan_mm(int64_t m, int64_t n, int64_t k, int sms) {
       const int per = int(ceil_div(kb, want)), splits = int(ceil_div(kb, per));
       const int64_t waves = ceil_div(tiles * splits, workers);
       double cost = double(waves) * (per * t.step + 1000) + 3000;
-      if (splits > 1) cost += 4000 + double(splits) * double(m) * double(n) * 8 / 2000;
+      if (splits > 1) cost += 6000 + double(splits) * double(m) * double(n) * 8 / 2000;
       if (best.bn == 0 || cost < best_cost) {
         best_cost = cost;
         best = {t.bn, t.g, splits, kb, per, splits > 1 ? int64_t(splits) * m * round_up(n, 8) * 4 : 0};
@@ -381,21 +382,40 @@ struct Staged {
       copy = static_cast<T*>(c.take(rows * stride * int64_t(sizeof(T))));
     }
   }
-  Operand ready(bool mn_major, const OpsDevice& d, cudaStream_t s) const {
-    if (!copy) return {src, stride, mn_major};
-    const int64_t vecs = rows * stride / kVec<T>;
-    dense_align_kernel<T><<<unsigned(std::min<int64_t>(ceil_div(vecs, 256), int64_t(d.sms) * 16)), 256, 0, s>>>(
-        static_cast<const T*>(src), src_stride, copy, stride, rows, cols);
-    check_launch("aligned copy");
-    return {copy, stride, mn_major};
+  Operand operand(bool mn_major) const { return {copy ? copy : src, stride, mn_major}; }
+  void add_to(DenseAlign& a, const OpsDevice& d) const {
+    if (!copy) return;
+    const int i = a.count++;
+    a.src[i] = src, a.dst[i] = copy, a.src_stride[i] = src_stride, a.dst_stride[i] = stride;
+    a.rows[i] = rows, a.cols[i] = cols;
+    a.first[i + 1] =
+        a.first[i] + unsigned(std::min<int64_t>(ceil_div(rows * stride / kVec<T>, 256), int64_t(d.sms) * 16));
   }
 };
+// The copies that staged matrices need, in one launch.
+template <class T, class... S>
+void align(const OpsDevice& d, cudaStream_t s, const S&... staged) {
+  static_assert(sizeof...(S) <= DenseAlign::MAX, "matrices a launch copies");
+  DenseAlign a{};
+  (staged.add_to(a, d), ...);
+  if (a.count == 0) return;
+  dense_align_kernel<T><<<a.first[a.count], 256, 0, s>>>(a);
+  check_launch("aligned copies");
+}
 
-constexpr int kRowsMax = 8;  // rows the FMA kernel takes
+// Whether a product goes through the FMA kernel: one or two rows, up to four
+// where the matrix of weights is small, up to eight where it is tiny. (bf16, m x k x
+// n, FMA against tensor cores: 1 x 4096 x 16384 27 us against 32, 4 x 4096 x 16384 35
+// against 32, 4 x 4096 x 4096 16.0 against 16.7, 4 x 8192 x 1024 10 against 14, 8 x
+// 8192 x 1024 18 against 14; of GPU time alone, 8 x 1024 x 1024 4.5 against 7.6.)
+inline bool few_rows(const mx_dense_args& a) {
+  const int64_t weights = a.k * a.n;
+  return a.m <= 2 || (a.m <= 4 && weights <= (int64_t(1) << 24)) || (a.m <= 8 && weights <= (int64_t(1) << 20));
+}
 
 template <class T>
 int64_t dense_workspace(const mx_dense_args& a, const OpsDevice& d) {
-  if (a.m <= kRowsMax) return 0;
+  if (few_rows(a)) return 0;
   Carver c{nullptr};
   Staged<T> x(c, a.x, a.x_stride, a.m, a.k), w(c, a.w, a.w_stride, a.n, a.k);
   c.take(plan_mm<T>(a.m, a.n, a.k, d.sms).part_bytes);
@@ -412,9 +432,12 @@ void dense_rows(const mx_dense_args& a, const DenseEpi& epi, const OpsDevice& d,
   const int64_t vecs = ceil_div(a.k, (vec ? kVec<T> : 1) * 32);
   int ks = 1;
   while (ks < 8 && ks < vecs && ceil_div(a.n, cpw) * ks < int64_t(d.sms) * 16) ks *= 2;
-  const unsigned grid = unsigned(ceil_div(ceil_div(a.n, cpw), 8 / ks));
+  // Small blocks spread evenly: 16384 columns over 148 SMs are 3.46 blocks of
+  // eight warps each, 6.92 of four.
+  const int warps = std::max(4, ks);
+  const unsigned grid = unsigned(ceil_div(ceil_div(a.n, cpw), warps / ks));
   auto go = [&](auto r, auto v, auto c) {
-    dense_rows_kernel<T, decltype(r)::value, decltype(v)::value, decltype(c)::value><<<grid, 256, 0, s>>>(
+    dense_rows_kernel<T, decltype(r)::value, decltype(v)::value, decltype(c)::value><<<grid, warps * 32, 0, s>>>(
         static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.w), a.w_stride, epi, int(a.m), int(a.n),
         int(a.k), ks);
   };
@@ -432,6 +455,8 @@ void dense_rows(const mx_dense_args& a, const DenseEpi& epi, const OpsDevice& d,
   };
   if (a.m == 1)
     by_vec(std::integral_constant<int, 1>());
+  else if (a.m == 2)
+    by_vec(std::integral_constant<int, 2>());
   else if (a.m <= 4)
     by_vec(std::integral_constant<int, 4>());
   else
@@ -449,13 +474,13 @@ void dense(const mx_dense_args& a, const OpsDevice& d, cudaStream_t s) {
   e.vec_y = aligned<T>(a.y, a.y_stride);
   e.vec_pre = a.pre && aligned<T>(a.pre, a.pre_stride);
   e.vec_bias = a.bias && aligned<T>(a.bias, 0);
-  if (a.m <= kRowsMax) return dense_rows<T>(a, e, d, s);
+  if (few_rows(a)) return dense_rows<T>(a, e, d, s);
   Carver c{static_cast<uint8_t*>(a.workspace)};
   Staged<T> x(c, a.x, a.x_stride, a.m, a.k), w(c, a.w, a.w_stride, a.n, a.k);
   const MmPlan plan = plan_mm<T>(a.m, a.n, a.k, d.sms);
   void* part = c.take(plan.part_bytes);
-  const Operand oa = x.ready(false, d, s), ob = w.ready(false, d, s);
-  run_mm<T>(oa, ob, a.m, a.n, a.k, e, plan, part, d, s);
+  align<T>(d, s, x, w);
+  run_mm<T>(x.operand(false), w.operand(false), a.m, a.n, a.k, e, plan, part, d, s);
 }
 
 // The pieces of the backward pass and where they lie in the workspace.
@@ -463,7 +488,8 @@ template <class T>
 struct DenseBackward {
   const bool act, products;
   bool vec;               // 16-byte accesses to dy, pre and d
-  int64_t chunks;         // row ranges of the column sums
+  int lx_log2;            // the column sums' blocks: 1 << lx_log2 threads across,
+  int64_t cols, chunks;   // cols x chunks of them
   T* d;                   // dy act'(pre), rounded to T
   int64_t d_stride;
   float* db_part;
@@ -471,7 +497,7 @@ struct DenseBackward {
   MmPlan dx, dw;
   void* part;
   DenseBackward(Carver& c, const mx_dense_backward_args& a, const OpsDevice& dev)
-      : act(a.act != MX_ACT_NONE), products(a.dx || a.dw), vec(false), chunks(0),
+      : act(a.act != MX_ACT_NONE), products(a.dx || a.dw), vec(false), lx_log2(5), cols(0), chunks(0),
         d(nullptr), d_stride(round_up(a.n, kVec<T>)), db_part(nullptr),
         // Without an activation d is dy itself.
         dy(c, act || !products ? nullptr : a.dy, act || !products ? 0 : a.dy_stride, a.m, a.n),
@@ -479,8 +505,10 @@ struct DenseBackward {
         w(c, a.dx ? a.w : nullptr, a.dx ? a.w_stride : 0, a.n, a.k), dx{}, dw{}, part(nullptr) {
     vec = aligned<T>(a.dy, a.dy_stride) && (!act || aligned<T>(a.pre, a.pre_stride)) && a.n % kVec<T> == 0;
     if (act || a.db) {
-      const int64_t cols = ceil_div(a.n, 32 * (vec ? kVec<T> : 1));
-      chunks = std::min<int64_t>(ceil_div(a.m, 16), std::max<int64_t>(1, int64_t(dev.sms) * 6 / cols));
+      const int64_t vecs = ceil_div(a.n, vec ? kVec<T> : 1);
+      while (lx_log2 > 0 && (int64_t(1) << (lx_log2 - 1)) >= vecs) --lx_log2;
+      cols = ceil_div(vecs, int64_t(1) << lx_log2);
+      chunks = std::min<int64_t>(ceil_div(a.m, 2 * (256 >> lx_log2)), std::max<int64_t>(1, int64_t(dev.sms) * 6 / cols));
     }
     if (act) d = static_cast<T*>(c.take(a.m * d_stride * int64_t(sizeof(T))));
     if (a.db) db_part = static_cast<float*>(c.take(chunks * a.n * 4));
@@ -510,9 +538,9 @@ void dense_backward(const mx_dense_backward_args& a, const OpsDevice& dev, cudaS
   if (b.act || a.db) {
     auto go = [&](auto v) {
       constexpr int V = decltype(v)::value;
-      dense_grad_kernel<T, V><<<dim3(unsigned(ceil_div(a.n, 32 * V)), unsigned(b.chunks)), 256, 0, s>>>(
+      dense_grad_kernel<T, V><<<dim3(unsigned(b.cols), unsigned(b.chunks)), 256, 0, s>>>(
           static_cast<const T*>(a.dy), a.dy_stride, static_cast<const T*>(a.pre), a.pre_stride, b.d, b.d_stride,
-          b.db_part, a.m, int(a.n), a.act, a.slope);
+          b.db_part, a.m, int(a.n), b.lx_log2, a.act, a.slope);
     };
     if (b.vec)
       go(std::integral_constant<int, kVec<T>>());
@@ -522,15 +550,16 @@ void dense_backward(const mx_dense_backward_args& a, const OpsDevice& dev, cudaS
     if (a.db) join_columns<T>(b.db_part, b.chunks, a.n, a.n, a.db, nullptr, false, s);
   }
   if (!b.products) return;
-  const Operand d = b.act ? Operand{b.d, b.d_stride, false} : b.dy.ready(false, dev, s);
+  align<T>(dev, s, b.dy, b.x, b.w);
+  const Operand d = b.act ? Operand{b.d, b.d_stride, false} : b.dy.operand(false);
   DenseEpi e{};
   if (a.dx) {
     e.y = a.dx, e.y_stride = a.dx_stride, e.vec_y = aligned<T>(a.dx, a.dx_stride);
-    run_mm<T>(d, b.w.ready(true, dev, s), a.m, a.k, a.n, e, b.dx, b.part, dev, s);
+    run_mm<T>(d, b.w.operand(true), a.m, a.k, a.n, e, b.dx, b.part, dev, s);
   }
   if (a.dw) {
     e.y = a.dw, e.y_stride = a.dw_stride, e.vec_y = aligned<T>(a.dw, a.dw_stride);
-    run_mm<T>({d.p, d.stride, true}, b.x.ready(true, dev, s), a.n, a.k, a.m, e, b.dw, b.part, dev, s);
+    run_mm<T>({d.p, d.stride, true}, b.x.operand(true), a.n, a.k, a.m, e, b.dw, b.part, dev, s);
   }
 }
 
