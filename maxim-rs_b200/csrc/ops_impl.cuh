@@ -204,11 +204,13 @@ struct MmPlan {
 };
 
 // Tile and number of splits of K: the cheapest by a model of the kernel's
-// time, in one SM's cycles. A k-block (128 bytes of K) of a tile costs `step`
-// cycles, a tile's first loads and last epilogue about 3000; the CTAs of the
-// slowest SM are what counts. Split sums cost their write and reading back
-// (about 2000 bytes a cycle for the whole GPU) and another launch (about 6000, most of
-// it the host's).
+// time, in one SM's cycles, its constants fitted to sweeps of all tiles and
+// splits over sizes from 64 x 512 x 512 to 20000 x 344 x 704 (the choice is within a few
+// percent of the best of each). A k-block (128 bytes of K) of a tile costs
+// `step` cycles, mostly its operands' way from the L2; a launch, its first
+// loads and last epilogue cost 7000; the CTAs of the slowest SM are what
+// counts. Split sums cost their write and reading back (2000 bytes a cycle
+// for the whole GPU) and another launch (5000).
 template <class T>
 MmPlan plan_mm(int64_t m, int64_t n, int64_t k, int sms) {
   constexpr bool F32 = sizeof(T) == 4;
@@ -217,8 +219,8 @@ MmPlan plan_mm(int64_t m, int64_t n, int64_t k, int sms) {
     int bn, g;
     double step;
   };
-  constexpr Tile kF32[] = {{64, 1, 1000}, {128, 1, 1500}, {128, 2, 1200}};
-  constexpr Tile k16[] = {{64, 1, 250}, {128, 1, 330}, {256, 1, 620}, {256, 2, 540}};
+  constexpr Tile kF32[] = {{64, 1, 1050}, {128, 1, 1570}, {128, 2, 1200}};
+  constexpr Tile k16[] = {{64, 1, 470}, {128, 1, 540}, {256, 1, 700}, {256, 2, 640}};
   MmPlan best{};
   double best_cost = 0;
   const int kb = int(ceil_div(k, BK));
@@ -226,17 +228,21 @@ MmPlan plan_mm(int64_t m, int64_t n, int64_t k, int sms) {
     const Tile& t = F32 ? kF32[i % 3] : k16[i];
     const int64_t tiles = ceil_div(m, 128 * t.g) * ceil_div(n, t.bn);
     const int workers = sms / t.g;
-    for (int want = 1; want <= kb; want = want < 8 ? want + 1 : want * 5 / 4) {
-      if (want > 1 && tiles * want > int64_t(workers) * 2) break;
+    auto consider = [&](int64_t want) {
+      if (want < 1 || want > kb || (want > 1 && tiles * want > int64_t(workers) * 2)) return;
       const int per = int(ceil_div(kb, want)), splits = int(ceil_div(kb, per));
       const int64_t waves = ceil_div(tiles * splits, workers);
-      double cost = double(waves) * (per * t.step + 1000) + 3000;
-      if (splits > 1) cost += 6000 + double(splits) * double(m) * double(n) * 8 / 2000;
+      double cost = double(waves) * (per * t.step + 1000) + 7000;
+      if (splits > 1) cost += 5000 + double(splits) * double(m) * double(n) * 8 / 2000;
       if (best.bn == 0 || cost < best_cost) {
         best_cost = cost;
         best = {t.bn, t.g, splits, kb, per, splits > 1 ? int64_t(splits) * m * round_up(n, 8) * 4 : 0};
       }
-    }
+    };
+    for (int want = 1; want <= 8; ++want) consider(want);
+    for (int want = 10; want < workers; want = want * 5 / 4) consider(want);
+    consider(workers / tiles);  // one full wave, or two
+    consider(2 * workers / tiles);
   }
   return best;
 }
