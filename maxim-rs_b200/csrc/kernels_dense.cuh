@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(256) dense_align_kernel(const __grid_constant_
 // loads 128 rows of A and BN / G rows of B and holds 128 accumulator rows. A
 // pair reads every B row into shared memory once for 256 rows of A: the
 // operands' way through shared memory is what bounds the one-CTA form
-// (8192 x 4096 -> 8192 bf16: 482 us with one, PAIRUS with two).
+// (8192 x 4096 -> 8192 bf16: 418 us with one CTA a tile, 363 with two).
 // One CTA per SM, persistent over the tiles. Warp roles:
 //   warp 0       TMA producer: 128 bytes of K (64 or 32 elements) a stage
 //   warp 1       MMA issuer (one lane, of the pair's leader)
@@ -357,10 +357,11 @@ __global__ void __launch_bounds__(256) dense_align_kernel(const __grid_constant_
 //                warps write lo = x - hi to a ring beside it)
 // Two accumulator sets let the epilogue of one tile overlap the products of
 // the next. In fp32 a set is two regions, hi*hi and the cross terms
-// hi*lo + lo*hi, and the epilogue takes a set every kChunk k-blocks and adds
+// hi*lo + lo*hi, and the epilogue takes a set every CHUNK k-blocks and adds
 // it up in registers: the tensor core truncates its accumulator at each MMA,
 // which over a few hundred of them costs more than the products' own rounding
-// (a sum of 1,900 in one set was off by 2.8e-6 of its size, of 256 by CHUNKERR).
+// (the weights' gradient over 71,680 rows was off by 2.8e-6 of its size with
+// 1,900 rows to a set, by 6.9e-7 with 256).
 // Every wait is bounded in time; one that runs out records a code in the
 // status word, and the kernel drains its copies and MMAs, frees its TMEM and
 // returns.
@@ -425,7 +426,7 @@ __device__ __forceinline__ float dense_residual(float v) {
 // tensor map and leaves by TMA, which also clips it to the matrix. (Where K is
 // short the epilogue sets the pace, by its warps' instruction latency: 71680 x
 // 128 -> 256 fp32 with GELU and pre took 58-70 us with the block read back and
-// stored by the lanes of 8 warps, 48 with TMA, EPINEW with 16 warps.) Matrices
+// stored by the lanes of 8 warps, 48 with TMA, 42 with 16 warps.) Matrices
 // that a tensor map cannot take (unaligned rows) are written by the lanes, a
 // column a lane.
 template <class T>
@@ -523,8 +524,9 @@ struct DenseOut {
     }
     put(static_cast<T*>(e.y), e.y_stride, e.vec_y, ty, v, row0, col0);
   }
+  // Before the block's shared memory goes: the stores have read it.
   __device__ __forceinline__ void done() const {
-    if (lane == 0) sm100::bulk_wait<0>();
+    if (lane == 0) sm100::bulk_wait_read<0>();
     __syncwarp();
   }
 };

@@ -145,7 +145,9 @@ def layer_norm(x, scale, bias, eps=1e-6, stats=False):
         _launch("mx_layer_norm", _NORM, (xp, scale.data_ptr(), bias.data_ptr(), y.data_ptr(), 0, 0, rows, c, xs, c,
                                          code, _DT[pt], eps, 0), device)
         return y
-    mean = x.new_empty(shape[:-1], dtype=torch.float32)
+    # new_empty without a dtype is the quicker call; any fp32 tensor at hand serves.
+    f32 = x if x.dtype is torch.float32 else scale
+    mean = f32.new_empty(shape[:-1]) if f32.dtype is torch.float32 else x.new_empty(shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     _launch("mx_layer_norm", _NORM, (xp, scale.data_ptr(), bias.data_ptr(), y.data_ptr(), mean.data_ptr(),
                                      rstd.data_ptr(), rows, c, xs, c, code, _DT[pt], eps, 0), device)
