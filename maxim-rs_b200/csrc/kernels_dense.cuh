@@ -260,8 +260,9 @@ __global__ void __launch_bounds__(256)
 template <class T, int V>
 __global__ void __launch_bounds__(256, 3)
     dense_grad_kernel(const T* dy, int64_t dy_stride, const T* pre, int64_t pre_stride, T* d, int64_t d_stride,
-                      float* part, int64_t m, int n, int lx_log2, int act, float slope) {
+                      float* part, T* db, int64_t m, int n, int lx_log2, int act, float slope) {
   __shared__ float sums[256 * V];
+  __shared__ float total[32 * V];
   const int lx = 1 << lx_log2, subs = 256 >> lx_log2;
   const int lane = threadIdx.x & (lx - 1), sub = threadIdx.x >> lx_log2;
   const int col = (blockIdx.x * lx + lane) * V;
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(256, 3)
       }
     }
   }
-  if (!part) return;
+  if (!part && !db) return;
 #pragma unroll
   for (int k = 0; k < V; ++k) sums[sub * lx * V + lane * V + k] = a[k];
   __syncthreads();
@@ -306,8 +307,24 @@ __global__ void __launch_bounds__(256, 3)
     float t = 0.0f;
 #pragma unroll 8
     for (int g = 0; g < subs; ++g) t += sums[g * lx * V + i];
-    part[int64_t(blockIdx.y) * n + cc] = t;
+    if (part)
+      part[int64_t(blockIdx.y) * n + cc] = t;
+    else
+      total[i] = t;
   }
+  if (part) return;
+  // A few rows: the row ranges are one cluster, whose first block adds their sums.
+  sm100::cluster_sync_all();
+  if (blockIdx.y == 0) {
+    for (int i = threadIdx.x; i < lx * V; i += 256) {
+      const int cc = blockIdx.x * lx * V + i;
+      if (cc >= n) continue;
+      float t = 0.0f;
+      for (unsigned b = 0; b < gridDim.y; ++b) t += sm100::cluster_ld(sm100::map_rank(&total[i], b));
+      db[cc] = from_f<T>(t);
+    }
+  }
+  sm100::cluster_sync_all();  // no block leaves while its sums are read
 }
 
 // Copies of matrices whose rows are not 16-byte aligned into ones whose rows

@@ -31,6 +31,21 @@ inline void check_launch(const char* what) {
   if (e != cudaSuccess) throw Error(std::string(what) + ": launch: " + cudaGetErrorString(e), MX_E_CUDA);
 }
 
+// A launch in clusters of the given shape (1 x 1 x 1: a plain one).
+template <class... P, class... A>
+void launch_clusters(void (*kernel)(P...), dim3 grid, dim3 block, int smem, dim3 cluster, cudaStream_t s, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid, cfg.blockDim = block;
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster.x, at[0].val.clusterDim.y = cluster.y, at[0].val.clusterDim.z = cluster.z;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 1 : 0;
+  MX_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
+}
+
 // ------------------------------------------------------------- layer norm
 // The lanes a row is spread over (L) and the vectors a lane holds (NV): the
 // fewest lanes that hold the row in 8 values each, up to a warp (fewer lanes
@@ -66,26 +81,33 @@ bool with_norm_shape(int c, F&& f) {
 }
 
 // Blocks of a kernel that one SM holds at once, asked once per kernel and
-// device, with the opt-in for its shared memory.
+// device, with the opt-in for its shared memory (`smem`, and `extra` where a launch takes more).
 template <class K>
-int resident_blocks(K* kernel, int threads, int smem, std::mutex& mu, int (&known)[64]) {
+int resident_blocks(K* kernel, int threads, int smem, int extra, std::mutex& mu, int (&known)[64]) {
   int dev = 0;
   MX_CUDA(cudaGetDevice(&dev));
   std::lock_guard<std::mutex> lock(mu);
   if (!known[dev]) {
-    MX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    MX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem + extra));
     MX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&known[dev], kernel, threads, smem));
   }
   return std::max(1, known[dev]);
 }
+// A few rows' parameter gradients are summed by one cluster: up to kClusterRows
+// rows for each group of lanes of each of its (at most 8) blocks, rows of up to
+// kClusterCols.
+constexpr int64_t kClusterRows = 10, kClusterCols = 4096;
+constexpr int kClusterSmem = int(2 * kClusterCols * 4);
+
 template <class T, int V, int L, int NV, bool BACKWARD>
 int norm_resident() {
   static std::mutex mu;
   static int known[64] = {};
   if constexpr (BACKWARD)
-    return resident_blocks(layer_norm_backward_kernel<T, V, L, NV>, kNormThreads<L>, kNormSmem<V, L, NV, 2>, mu, known);
+    return resident_blocks(layer_norm_backward_kernel<T, V, L, NV>, kNormThreads<L>, kNormSmem<V, L, NV, 2>,
+                           kClusterSmem, mu, known);
   else
-    return resident_blocks(layer_norm_kernel<T, V, L, NV>, kNormThreads<L>, kNormSmem<V, L, NV, 1>, mu, known);
+    return resident_blocks(layer_norm_kernel<T, V, L, NV>, kNormThreads<L>, kNormSmem<V, L, NV, 1>, 0, mu, known);
 }
 
 template <class T, int V>
@@ -116,33 +138,42 @@ bool norm_backward_vec(const mx_layer_norm_backward_args& a) {
          a.c % kVec<T> == 0;
 }
 // Blocks of the backward kernel, which is also how many partial rows of the
-// parameter gradients it leaves.
+// parameter gradients it leaves; or those of one cluster, which leaves none.
+struct NormBlocks {
+  int64_t blocks;
+  bool cluster;
+};
 template <class T, int V>
-int64_t norm_backward_blocks(const mx_layer_norm_backward_args& a, const OpsDevice& d) {
-  int64_t blocks = 0;
+NormBlocks norm_backward_blocks(const mx_layer_norm_backward_args& a, const OpsDevice& d) {
+  NormBlocks n{0, false};
   const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto nv) {
-    constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
-    blocks = std::min<int64_t>(ceil_div(a.rows, kNormThreads<L> / L), int64_t(d.sms) * norm_resident<T, V, L, NV, true>());
+    constexpr int L = decltype(l)::value, NV = decltype(nv)::value, GROUPS = kNormThreads<L> / L;
+    const int resident = norm_resident<T, V, L, NV, true>();
+    const int64_t want = ceil_div(a.rows, GROUPS);
+    n.cluster = (a.dscale || a.dbias) && want <= 8 * kClusterRows && a.c <= kClusterCols;
+    n.blocks = n.cluster ? std::min<int64_t>(want, 8) : std::min<int64_t>(want, int64_t(d.sms) * resident);
   });
-  if (!done) blocks = std::min<int64_t>(ceil_div(a.rows, 8), std::max<int64_t>(1, d.sms * 4 / ceil_div(a.c, 32 * V)));
-  return blocks;
+  if (!done) n.blocks = std::min<int64_t>(ceil_div(a.rows, 8), std::max<int64_t>(1, d.sms * 4 / ceil_div(a.c, 32 * V)));
+  return n;
 }
 
 template <class T, int V>
 void norm_backward_v(const mx_layer_norm_backward_args& a, const OpsDevice& d, cudaStream_t s) {
-  const int64_t blocks = norm_backward_blocks<T, V>(a, d);
-  float* part = a.dscale || a.dbias ? static_cast<float*>(a.workspace) : nullptr;
-  NormBwd p{a.dy, a.x, a.scale, a.mean, a.rstd, a.dx, part, a.rows, a.dy_stride, a.x_stride, a.dx_stride,
-            int(a.c), a.param_dtype == MX_DT_F32};
+  const NormBlocks n = norm_backward_blocks<T, V>(a, d);
+  float* part = (a.dscale || a.dbias) && !n.cluster ? static_cast<float*>(a.workspace) : nullptr;
+  NormBwd p{a.dy, a.x, a.scale, a.mean, a.rstd, a.dx, part, n.cluster ? int(n.blocks) : 0, a.dscale, a.dbias,
+            a.rows, a.dy_stride, a.x_stride, a.dx_stride, int(a.c), a.param_dtype == MX_DT_F32};
   const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto nv) {
     constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
-    layer_norm_backward_kernel<T, V, L, NV><<<unsigned(blocks), kNormThreads<L>, kNormSmem<V, L, NV, 2>, s>>>(p);
+    const int smem = kNormSmem<V, L, NV, 2> + (n.cluster ? int(2 * a.c * 4) : 0);
+    launch_clusters(layer_norm_backward_kernel<T, V, L, NV>, dim3(unsigned(n.blocks)), dim3(kNormThreads<L>), smem,
+                    n.cluster ? dim3(unsigned(n.blocks)) : dim3(1), s, p);
   });
   if (!done) {
     // The sums first: dx may overwrite dy.
     if (part)
       layer_norm_param_long_kernel<T, V>
-          <<<dim3(unsigned(ceil_div(a.c, 32 * V)), unsigned(blocks)), 256, 0, s>>>(p);
+          <<<dim3(unsigned(ceil_div(a.c, 32 * V)), unsigned(n.blocks)), 256, 0, s>>>(p);
     if (a.dx)
       layer_norm_dx_long_kernel<T, V><<<unsigned(std::min<int64_t>(a.rows, int64_t(d.sms) * 4)), 512, 0, s>>>(p);
   }
@@ -162,10 +193,15 @@ void join_columns(const float* part, int64_t nb, int64_t cols, int64_t split, vo
 }
 
 template <class T>
+NormBlocks norm_backward_plan(const mx_layer_norm_backward_args& a, const OpsDevice& d) {
+  return norm_backward_vec<T>(a) ? norm_backward_blocks<T, kVec<T>>(a, d) : norm_backward_blocks<T, 1>(a, d);
+}
+
+template <class T>
 int64_t layer_norm_backward_workspace(const mx_layer_norm_backward_args& a, const OpsDevice& d) {
-  if (!a.dscale && !a.dbias) return 0;
-  const int64_t blocks = norm_backward_vec<T>(a) ? norm_backward_blocks<T, kVec<T>>(a, d) : norm_backward_blocks<T, 1>(a, d);
-  return blocks * 2 * a.c * 4;
+  if ((!a.dscale && !a.dbias) || a.rows == 0) return 0;
+  const NormBlocks n = norm_backward_plan<T>(a, d);
+  return n.cluster ? 0 : n.blocks * 2 * a.c * 4;
 }
 
 template <class T>
@@ -177,15 +213,13 @@ void layer_norm_backward(const mx_layer_norm_backward_args& a, const OpsDevice& 
     if (a.dbias) MX_CUDA(cudaMemsetAsync(a.dbias, 0, bytes, s));
     return;
   }
-  const bool vec = norm_backward_vec<T>(a);
-  if (vec)
+  if (norm_backward_vec<T>(a))
     norm_backward_v<T, kVec<T>>(a, d, s);
   else
     norm_backward_v<T, 1>(a, d, s);
-  if (a.dscale || a.dbias)
-    join_columns<T>(static_cast<const float*>(a.workspace),
-                    vec ? norm_backward_blocks<T, kVec<T>>(a, d) : norm_backward_blocks<T, 1>(a, d), 2 * a.c, a.c, a.dscale,
-                    a.dbias, out_f32, s);
+  const NormBlocks n = norm_backward_plan<T>(a, d);
+  if ((a.dscale || a.dbias) && !n.cluster)
+    join_columns<T>(static_cast<const float*>(a.workspace), n.blocks, 2 * a.c, a.c, a.dscale, a.dbias, out_f32, s);
 }
 
 // ------------------------------------------------------------------ dense
@@ -310,17 +344,8 @@ void launch_mm(const Operand& a, const Operand& b, const DenseMm& p, int64_t k, 
   const CUtensorMap tpre =
       !p.epi.part && p.epi.vec_pre ? result_map<T>(p.epi.pre, p.epi.pre_stride, p.m, p.n, 1) : CUtensorMap{};
   const int64_t items = int64_t(p.tiles_m) * p.tiles_n * p.splits;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(std::min<int64_t>(items, d.sms / G) * G));
-  cfg.blockDim = dim3(C::THREADS);
-  cfg.dynamicSmemBytes = C::SMEM_BYTES;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = G, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = G == 2 ? 1 : 0;
-  MX_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, ty, tpre, p));
+  launch_clusters(kernel, dim3(unsigned(std::min<int64_t>(items, d.sms / G) * G)), dim3(C::THREADS), C::SMEM_BYTES,
+                  dim3(G), s, ta, tb, ty, tpre, p);
 }
 
 // D = A B^T with the epilogue `epi`: the product, and the join of its splits.
@@ -495,7 +520,8 @@ struct DenseBackward {
   const bool act, products;
   bool vec;               // 16-byte accesses to dy, pre and d
   int lx_log2;            // the column sums' blocks: 1 << lx_log2 threads across,
-  int64_t cols, chunks;   // cols x chunks of them
+  int64_t cols, chunks;   // cols x chunks of them,
+  bool cluster;           // the chunks as one cluster
   T* d;                   // dy act'(pre), rounded to T
   int64_t d_stride;
   float* db_part;
@@ -503,7 +529,7 @@ struct DenseBackward {
   MmPlan dx, dw;
   void* part;
   DenseBackward(Carver& c, const mx_dense_backward_args& a, const OpsDevice& dev)
-      : act(a.act != MX_ACT_NONE), products(a.dx || a.dw), vec(false), lx_log2(5), cols(0), chunks(0),
+      : act(a.act != MX_ACT_NONE), products(a.dx || a.dw), vec(false), lx_log2(5), cols(0), chunks(0), cluster(false),
         d(nullptr), d_stride(round_up(a.n, kVec<T>)), db_part(nullptr),
         // Without an activation d is dy itself.
         dy(c, act || !products ? nullptr : a.dy, act || !products ? 0 : a.dy_stride, a.m, a.n),
@@ -514,10 +540,15 @@ struct DenseBackward {
       const int64_t vecs = ceil_div(a.n, vec ? kVec<T> : 1);
       while (lx_log2 > 0 && (int64_t(1) << (lx_log2 - 1)) >= vecs) --lx_log2;
       cols = ceil_div(vecs, int64_t(1) << lx_log2);
-      chunks = std::min<int64_t>(ceil_div(a.m, 2 * (256 >> lx_log2)), std::max<int64_t>(1, int64_t(dev.sms) * 6 / cols));
+      // Up to 16 rows a thread in 8 blocks: one cluster joins the sums itself
+      // (another launch would cost more).
+      const int64_t subs = 256 >> lx_log2;
+      cluster = a.db && a.m <= 8 * 16 * subs;
+      chunks = cluster ? std::min<int64_t>(8, ceil_div(a.m, 2 * subs))
+                       : std::min<int64_t>(ceil_div(a.m, 2 * subs), std::max<int64_t>(1, int64_t(dev.sms) * 6 / cols));
     }
     if (act) d = static_cast<T*>(c.take(a.m * d_stride * int64_t(sizeof(T))));
-    if (a.db) db_part = static_cast<float*>(c.take(chunks * a.n * 4));
+    if (a.db && !cluster) db_part = static_cast<float*>(c.take(chunks * a.n * 4));
     if (a.dx) dx = plan_mm<T>(a.m, a.k, a.n, dev.sms);
     if (a.dw) dw = plan_mm<T>(a.n, a.k, a.m, dev.sms);
     part = c.take(std::max(dx.part_bytes, dw.part_bytes));  // the products run one after the other
@@ -544,16 +575,17 @@ void dense_backward(const mx_dense_backward_args& a, const OpsDevice& dev, cudaS
   if (b.act || a.db) {
     auto go = [&](auto v) {
       constexpr int V = decltype(v)::value;
-      dense_grad_kernel<T, V><<<dim3(unsigned(b.cols), unsigned(b.chunks)), 256, 0, s>>>(
-          static_cast<const T*>(a.dy), a.dy_stride, static_cast<const T*>(a.pre), a.pre_stride, b.d, b.d_stride,
-          b.db_part, a.m, int(a.n), b.lx_log2, a.act, a.slope);
+      launch_clusters(dense_grad_kernel<T, V>, dim3(unsigned(b.cols), unsigned(b.chunks)), dim3(256), 0,
+                      b.cluster ? dim3(1, unsigned(b.chunks)) : dim3(1), s, static_cast<const T*>(a.dy), a.dy_stride,
+                      static_cast<const T*>(a.pre), a.pre_stride, b.d, b.d_stride, b.db_part,
+                      b.cluster ? static_cast<T*>(a.db) : nullptr, a.m, int(a.n), b.lx_log2, int(a.act), a.slope);
     };
     if (b.vec)
       go(std::integral_constant<int, kVec<T>>());
     else
       go(std::integral_constant<int, 1>());
     check_launch("mx_dense_backward");
-    if (a.db) join_columns<T>(b.db_part, b.chunks, a.n, a.n, a.db, nullptr, false, s);
+    if (b.db_part) join_columns<T>(b.db_part, b.chunks, a.n, a.n, a.db, nullptr, false, s);
   }
   if (!b.products) return;
   align<T>(dev, s, b.dy, b.x, b.w);

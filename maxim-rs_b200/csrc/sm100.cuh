@@ -85,9 +85,9 @@ __device__ __forceinline__ bool elect_one() {
   return on != 0;
 }
 
-// ---------------------------------------------------------- CTA pairs
-// Two CTAs of a cluster that work on one tile (cta_group::2). A barrier of
-// the pair's leader is reached through its shared::cluster address.
+// ------------------------------------------------------------ clusters
+// The CTAs of a cluster reach one another's shared memory by its
+// shared::cluster address; a pair of them works on one tile (cta_group::2).
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -98,6 +98,12 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
 }
+__device__ __forceinline__ float cluster_ld(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+// Every thread of every CTA of the cluster; writes before it are visible after it.
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
