@@ -377,9 +377,9 @@ __global__ void __launch_bounds__(256) dense_align_kernel(const __grid_constant_
 //                the fp32 tile itself is hi, read truncated to TF32; these
 //                warps write lo = x - hi to a ring beside it)
 // Two accumulator sets let the epilogue of one tile overlap the products of
-// the next. In fp32 a set is two regions, hi*hi and the cross terms
-// hi*lo + lo*hi, and the epilogue takes a set every CHUNK k-blocks and adds
-// it up in registers: the tensor core truncates its accumulator at each MMA,
+// the next. In fp32 the cross terms hi*lo + lo*hi have a region of their own in
+// a set where TMEM has room for it, and the epilogue takes a set every CHUNK
+// k-blocks and adds it up in registers: the tensor core truncates its accumulator at each MMA,
 // which over a few hundred of them costs more than the products' own rounding
 // (the weights' gradient over 71,680 rows was off by 2.8e-6 of its size with
 // 1,900 rows to a set, by 6.9e-7 with 256).
@@ -411,13 +411,21 @@ struct DenseCfg {
   static constexpr int LO_STAGES = F32 ? 2 : 0;
   static constexpr int FIT = 192 * 1024 / STAGE_BYTES - LO_STAGES;
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
-  static constexpr int SET_COLS = F32 ? 2 * BN : BN;
+  static constexpr int REGIONS = F32 && BN <= 128 ? 2 : 1;  // of an accumulator set: hi*hi and the cross terms, or one
+  static constexpr int SET_COLS = REGIONS * BN;
   static constexpr int TMEM_COLS = 2 * SET_COLS;
-  static constexpr int CHUNK = F32 ? 8 : 1 << 30;  // k-blocks a set accumulates
+  // k-blocks a set accumulates: 32 updates of hi*hi, or 24 of everything.
+  static constexpr int CHUNK = !F32 ? 1 << 30 : (REGIONS == 2 ? 8 : 2);
   static constexpr int EPI_WARP0 = 4, EPI_WARPS = BN >= 128 ? 16 : 8;
   static constexpr int EPI_COLS = BN / (EPI_WARPS / 4);  // columns of a tile per epilogue warp
   static constexpr int SPLIT_WARP0 = EPI_WARP0 + EPI_WARPS, SPLIT_WARPS = F32 ? 4 : 0;
   static constexpr int THREADS = 32 * (SPLIT_WARP0 + SPLIT_WARPS);
+  // fp32 with BN = 256: an epilogue lane's 64 sums need more registers than the
+  // 80 that 768 threads launch with, the other warps less. In the six
+  // warpgroups' sum: 40 + 4 x 96 + 48 = 472 of 480.
+  static constexpr bool SPLIT_REGS = F32 && BN == 256;
+  static constexpr int REGS_CONTROL = 40, REGS_EPI = 96, REGS_SPLIT = 48;
+  static_assert(!SPLIT_REGS || (THREADS == 768 && REGS_CONTROL + 4 * REGS_EPI + REGS_SPLIT <= 480), "register split");
   static constexpr int STAGING_BYTES = EPI_WARPS * 2048;  // 32 rows x 64 bytes each
   static constexpr int SMEM_BYTES = 1024 + (STAGES + LO_STAGES) * STAGE_BYTES + STAGING_BYTES + 8 * (2 * STAGES + 2 * LO_STAGES + 5) + 16;
   static_assert(SMEM_BYTES <= 232448 - 64, "shared memory per CTA");
@@ -633,143 +641,148 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
       mma_commit(bar);
   };
 
-  if (warp == 0) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      for (int w = first; w < items && !*vabort; w += step) {
-        int tm, tn, k0, k1;
-        dense_tile(p, w % tiles, tm, tn);
-        kb_range(w / tiles, k0, k1);
-        const int row = (tm * G + rank) * 128, col = tn * BN + rank * C::BROWS;
-        for (int kb = k0; kb < k1; ++kb, ++it) {
-          const int s = it % C::STAGES;
-          if (!wait(&empty[s], ((it / C::STAGES) & 1) ^ 1)) {
-            fail(kDenseErrProducer);
-            break;
-          }
-          uint8_t* a = base + s * C::STAGE_BYTES;
-          uint8_t* b = a + C::A_BYTES;
-          // 16-bit pair: both CTAs' bytes count on the leader's barrier, which
-          // the MMA issuer waits on. In fp32 each CTA's split warps wait on
-          // their own.
-          constexpr bool SHARED = G == 2 && !C::F32;
-          if (!SHARED || rank == 0) mbar_arrive_expect_tx(&full[s], (SHARED ? 2 : 1) * (C::A_BYTES + C::B_BYTES));
-          const uint32_t leader_full = SHARED ? map_rank(&full[s], 0) : 0;
-          auto load = [&](uint8_t* dst, const CUtensorMap* map, int c0, int c1) {
-            if constexpr (SHARED)
-              tma_load_2d_pair(dst, map, leader_full, c0, c1);
-            else
-              tma_load_2d(dst, map, &full[s], c0, c1);
-          };
-          // K-major: one box of the tile's rows x 128 bytes of K. MN-major: a box
-          // of BK rows of K x 128 bytes of M (N) for each 128 bytes of it.
-          if (A_MN) {
-#pragma unroll
-            for (int c = 0; c < 128 / C::BK; ++c) load(a + c * C::BK * 128, &tmA, row + c * C::BK, kb * C::BK);
-          } else {
-            load(a, &tmA, kb * C::BK, row);
-          }
-          if (B_MN) {
-#pragma unroll
-            for (int c = 0; c < C::BROWS / C::BK; ++c) load(b + c * C::BK * 128, &tmB, col + c * C::BK, kb * C::BK);
-          } else {
-            load(b, &tmB, kb * C::BK, col);
-          }
-        }
-      }
-      if (*vabort)  // copies in flight land before the CTA may leave
-        for (uint32_t j = it < C::STAGES ? 0 : it - C::STAGES; j < it; ++j)
-          if ((G == 2 && !C::F32 && rank != 0) || !wait(&full[j % C::STAGES], (j / C::STAGES) & 1)) break;
-    }
-  } else if (warp == 1) {
-    // The whole warp runs the loop, so that what the MMAs take is the same in
-    // all lanes and stays in uniform registers; one lane issues.
-    if (rank == 0) {
-      constexpr uint32_t idesc =
-          C::F32 ? idesc_tf32(128 * G, BN, A_MN, B_MN)
-                 : idesc_f16(128 * G, BN, A_MN, B_MN, std::is_same<T, __nv_bfloat16>::value ? 1 : 0);
-      // Steps of one MMA along K, in the descriptors' 16-byte units: 32 bytes
-      // of a K-major row, or 16 (8 in fp32) 128-byte rows of an MN-major tile.
-      constexpr uint32_t step_a = A_MN ? (C::F32 ? 64u : 128u) : 2u;
-      constexpr uint32_t step_b = B_MN ? (C::F32 ? 64u : 128u) : 2u;
-      auto desc = [](uint32_t addr, bool mn) {
-        if (!mn) return desc_kmajor_sw128(addr);
-        return C::F32 ? desc_mnmajor_sw128_32b(addr, C::BK * 128) : desc_mnmajor_sw128(addr, C::BK * 128);
-      };
-      auto mma = [](uint32_t d, uint64_t da, uint64_t db, uint32_t more) {
-        if constexpr (C::F32) {
-          if constexpr (G == 2)
-            mma_tf32_pair(d, da, db, idesc, more);
-          else
-            mma_tf32(d, da, db, idesc, more);
-        } else {
-          if constexpr (G == 2)
-            mma_f16_pair(d, da, db, idesc, more);
-          else
-            mma_f16(d, da, db, idesc, more);
-        }
-      };
-      const uint32_t base_u = smem_u32(base), lo_u = smem_u32(lo_base);
-      uint32_t s = 0, ph = 0, l = 0, lph = 0, tc = 0;
-      bool ok = true;
-      for (int w = first; w < items && ok; w += step) {
-        int k0, k1;
-        kb_range(w / tiles, k0, k1);
-        uint32_t d = 0;
-        int left = 0;  // k-blocks the accumulator set still takes
-        for (int kb = k0; kb < k1; ++kb) {
-          const bool fresh = left == 0;
-          if (fresh) {
-            const uint32_t acc = tc & 1;
-            ok = __all_sync(0xFFFFFFFFu, wait(&acc_empty[acc], ((tc >> 1) & 1) ^ 1));
-            if (!ok) {
-              if (lane == 0) fail(kDenseErrMmaAcc);
+  if (warp < C::EPI_WARP0) {
+    if constexpr (C::SPLIT_REGS) regs_dec<C::REGS_CONTROL>();
+    if (warp == 0) {
+      if (lane == 0) {
+        uint32_t it = 0;
+        for (int w = first; w < items && !*vabort; w += step) {
+          int tm, tn, k0, k1;
+          dense_tile(p, w % tiles, tm, tn);
+          kb_range(w / tiles, k0, k1);
+          const int row = (tm * G + rank) * 128, col = tn * BN + rank * C::BROWS;
+          for (int kb = k0; kb < k1; ++kb, ++it) {
+            const int s = it % C::STAGES;
+            if (!wait(&empty[s], ((it / C::STAGES) & 1) ^ 1)) {
+              fail(kDenseErrProducer);
               break;
             }
-            d = tmem + acc * C::SET_COLS;
-            left = min(C::CHUNK, k1 - kb);
-          }
-          ok = __all_sync(0xFFFFFFFFu, C::F32 ? wait(&lo_ready[l], lph) : wait(&full[s], ph));
-          if (!ok) {
-            if (lane == 0) fail(kDenseErrMmaStage);
-            break;
-          }
-          tc_fence_after();
-          const uint32_t a = base_u + s * C::STAGE_BYTES, b = a + C::A_BYTES;
-          const uint64_t da = desc(a, A_MN), db = desc(b, B_MN);
-          --left;
-          if (elect_one()) {
-            if constexpr (C::F32) {
-              const uint32_t alo = lo_u + l * C::STAGE_BYTES, blo = alo + C::A_BYTES;
-              const uint64_t dal = desc(alo, A_MN), dbl = desc(blo, B_MN);
+            uint8_t* a = base + s * C::STAGE_BYTES;
+            uint8_t* b = a + C::A_BYTES;
+            // 16-bit pair: both CTAs' bytes count on the leader's barrier, which
+            // the MMA issuer waits on. In fp32 each CTA's split warps wait on
+            // their own.
+            constexpr bool SHARED = G == 2 && !C::F32;
+            if (!SHARED || rank == 0) mbar_arrive_expect_tx(&full[s], (SHARED ? 2 : 1) * (C::A_BYTES + C::B_BYTES));
+            const uint32_t leader_full = SHARED ? map_rank(&full[s], 0) : 0;
+            auto load = [&](uint8_t* dst, const CUtensorMap* map, int c0, int c1) {
+              if constexpr (SHARED)
+                tma_load_2d_pair(dst, map, leader_full, c0, c1);
+              else
+                tma_load_2d(dst, map, &full[s], c0, c1);
+            };
+            // K-major: one box of the tile's rows x 128 bytes of K. MN-major: a box
+            // of BK rows of K x 128 bytes of M (N) for each 128 bytes of it.
+            if (A_MN) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t more = !fresh || k > 0;
-                mma(d, da + step_a * k, db + step_b * k, more);
-                mma(d + BN, da + step_a * k, dbl + step_b * k, more);
-                mma(d + BN, dal + step_a * k, db + step_b * k, 1u);
-              }
+              for (int c = 0; c < 128 / C::BK; ++c) load(a + c * C::BK * 128, &tmA, row + c * C::BK, kb * C::BK);
             } else {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) mma(d, da + step_a * k, db + step_b * k, !fresh || k > 0);
+              load(a, &tmA, kb * C::BK, row);
             }
-            commit(&empty[s]);
-            if constexpr (C::F32) commit(&lo_empty[l]);
-            if (left == 0) commit(&acc_full[tc & 1]);
+            if (B_MN) {
+#pragma unroll
+              for (int c = 0; c < C::BROWS / C::BK; ++c) load(b + c * C::BK * 128, &tmB, col + c * C::BK, kb * C::BK);
+            } else {
+              load(b, &tmB, kb * C::BK, col);
+            }
           }
+        }
+        if (*vabort)  // copies in flight land before the CTA may leave
+          for (uint32_t j = it < C::STAGES ? 0 : it - C::STAGES; j < it; ++j)
+            if ((G == 2 && !C::F32 && rank != 0) || !wait(&full[j % C::STAGES], (j / C::STAGES) & 1)) break;
+      }
+    } else if (warp == 1) {
+      // The whole warp runs the loop, so that what the MMAs take is the same in
+      // all lanes and stays in uniform registers; one lane issues.
+      if (rank == 0) {
+        constexpr uint32_t idesc =
+            C::F32 ? idesc_tf32(128 * G, BN, A_MN, B_MN)
+                   : idesc_f16(128 * G, BN, A_MN, B_MN, std::is_same<T, __nv_bfloat16>::value ? 1 : 0);
+        // Steps of one MMA along K, in the descriptors' 16-byte units: 32 bytes
+        // of a K-major row, or 16 (8 in fp32) 128-byte rows of an MN-major tile.
+        constexpr uint32_t step_a = A_MN ? (C::F32 ? 64u : 128u) : 2u;
+        constexpr uint32_t step_b = B_MN ? (C::F32 ? 64u : 128u) : 2u;
+        auto desc = [](uint32_t addr, bool mn) {
+          if (!mn) return desc_kmajor_sw128(addr);
+          return C::F32 ? desc_mnmajor_sw128_32b(addr, C::BK * 128) : desc_mnmajor_sw128(addr, C::BK * 128);
+        };
+        auto mma = [](uint32_t d, uint64_t da, uint64_t db, uint32_t more) {
+          if constexpr (C::F32) {
+            if constexpr (G == 2)
+              mma_tf32_pair(d, da, db, idesc, more);
+            else
+              mma_tf32(d, da, db, idesc, more);
+          } else {
+            if constexpr (G == 2)
+              mma_f16_pair(d, da, db, idesc, more);
+            else
+              mma_f16(d, da, db, idesc, more);
+          }
+        };
+        constexpr uint32_t CROSS = C::REGIONS == 2 ? BN : 0;  // the cross terms' columns
+        const uint32_t base_u = smem_u32(base), lo_u = smem_u32(lo_base);
+        uint32_t s = 0, ph = 0, l = 0, lph = 0, tc = 0;
+        bool ok = true;
+        for (int w = first; w < items && ok; w += step) {
+          int k0, k1;
+          kb_range(w / tiles, k0, k1);
+          uint32_t d = 0;
+          int left = 0;  // k-blocks the accumulator set still takes
+          for (int kb = k0; kb < k1; ++kb) {
+            const bool fresh = left == 0;
+            if (fresh) {
+              const uint32_t acc = tc & 1;
+              ok = __all_sync(0xFFFFFFFFu, wait(&acc_empty[acc], ((tc >> 1) & 1) ^ 1));
+              if (!ok) {
+                if (lane == 0) fail(kDenseErrMmaAcc);
+                break;
+              }
+              d = tmem + acc * C::SET_COLS;
+              left = min(C::CHUNK, k1 - kb);
+            }
+            ok = __all_sync(0xFFFFFFFFu, C::F32 ? wait(&lo_ready[l], lph) : wait(&full[s], ph));
+            if (!ok) {
+              if (lane == 0) fail(kDenseErrMmaStage);
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a = base_u + s * C::STAGE_BYTES, b = a + C::A_BYTES;
+            const uint64_t da = desc(a, A_MN), db = desc(b, B_MN);
+            --left;
+            if (elect_one()) {
+              if constexpr (C::F32) {
+                const uint32_t alo = lo_u + l * C::STAGE_BYTES, blo = alo + C::A_BYTES;
+                const uint64_t dal = desc(alo, A_MN), dbl = desc(blo, B_MN);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const uint32_t more = !fresh || k > 0;
+                  mma(d, da + step_a * k, db + step_b * k, more);
+                  mma(d + CROSS, da + step_a * k, dbl + step_b * k, C::REGIONS == 2 ? more : 1u);
+                  mma(d + CROSS, dal + step_a * k, db + step_b * k, 1u);
+                }
+              } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mma(d, da + step_a * k, db + step_b * k, !fresh || k > 0);
+              }
+              commit(&empty[s]);
+              if constexpr (C::F32) commit(&lo_empty[l]);
+              if (left == 0) commit(&acc_full[tc & 1]);
+            }
+            __syncwarp();
+            if (left == 0) ++tc;
+            if (++s == C::STAGES) s = 0, ph ^= 1;
+            if (C::F32 && ++l == C::LO_STAGES) l = 0, lph ^= 1;
+          }
+        }
+        if (!ok) {
+          if (elect_one()) commit(drained);
           __syncwarp();
-          if (left == 0) ++tc;
-          if (++s == C::STAGES) s = 0, ph ^= 1;
-          if (C::F32 && ++l == C::LO_STAGES) l = 0, lph ^= 1;
+          wait(drained, 0);
         }
       }
-      if (!ok) {
-        if (elect_one()) commit(drained);
-        __syncwarp();
-        wait(drained, 0);
-      }
     }
-  } else if (warp >= C::EPI_WARP0 && warp < C::EPI_WARP0 + C::EPI_WARPS) {
+  } else if (warp < C::SPLIT_WARP0) {
+    if constexpr (C::SPLIT_REGS) regs_inc<C::REGS_EPI>();
     const int ew = warp - C::EPI_WARP0, q = warp & 3, part = ew >> 2;
     DenseOut<T> out{p, &tmY, &tmPre, staging + ew * 2048, lane};
     uint32_t tc = 0;
@@ -795,24 +808,32 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
         ++tc;
       };
       if constexpr (C::F32) {
-        static_assert(!C::F32 || C::EPI_COLS == 32, "one block a warp");
-        float sum[32];
-        out.bias(col0, sum);
+        constexpr int COLS = C::EPI_COLS;
+        float sum[COLS];
+#pragma unroll
+        for (int c = 0; c < COLS; c += 32) out.bias(col0 + c, sum + c);
         for (int kb = k0; kb < k1 && ok; kb += C::CHUNK) {
           ok = take();
           if (!ok) break;
-          const uint32_t d = tmem + (uint32_t(q * 32) << 16) + (tc & 1) * C::SET_COLS + part * 32;
+          const uint32_t d = tmem + (uint32_t(q * 32) << 16) + (tc & 1) * C::SET_COLS + part * COLS;
 #pragma unroll
-          for (int c = 0; c < 32; c += 16) {
+          for (int c = 0; c < COLS; c += 16) {
             float hh[16], cross[16];
-            tmem_ld16x2(d + c, d + BN + c, hh, cross);
+            if constexpr (C::REGIONS == 2) {
+              tmem_ld16x2(d + c, d + BN + c, hh, cross);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sum[c + i] += hh[i] + cross[i];
+              for (int i = 0; i < 16; ++i) sum[c + i] += hh[i] + cross[i];
+            } else {
+              tmem_ld16(d + c, hh);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) sum[c + i] += hh[i];
+            }
           }
           give();
         }
         if (!ok) break;
-        out.finish(sum, split, row0, col0);
+#pragma unroll
+        for (int c = 0; c < COLS; c += 32) out.finish(sum + c, split, row0, col0 + c);
       } else {
         ok = take();
         if (!ok) break;
@@ -830,8 +851,8 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
       }
     }
     out.done();
-  }
-  if constexpr (C::F32) if (warp >= C::SPLIT_WARP0) {
+  } else if constexpr (C::F32) {
+    if constexpr (C::SPLIT_REGS) regs_dec<C::REGS_SPLIT>();
     const int tid = threadIdx.x - 32 * C::SPLIT_WARP0;
     uint32_t s = 0, ph = 0, l = 0, lph = 0;
     bool ok = true;
@@ -847,14 +868,19 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
         // Elementwise, so the swizzled layouts do not matter.
         const float4* src = reinterpret_cast<const float4*>(base + s * C::STAGE_BYTES) + tid;
         float4* dst = reinterpret_cast<float4*>(lo_base + l * C::STAGE_BYTES) + tid;
-        constexpr int STEP = 32 * C::SPLIT_WARPS, PER = C::F32 ? C::STAGE_BYTES / 16 / STEP : 1;
-        float4 v[PER];
+        constexpr int STEP = 32 * C::SPLIT_WARPS, PER = C::STAGE_BYTES / 16 / STEP;
+        constexpr int BATCH = C::SPLIT_REGS ? 4 : PER;  // loads ahead of their use
+        static_assert(PER % BATCH == 0, "whole batches");
 #pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] = src[i * STEP];
+        for (int j = 0; j < PER; j += BATCH) {
+          float4 v[BATCH];
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-          dst[i * STEP] = make_float4(dense_residual(v[i].x), dense_residual(v[i].y), dense_residual(v[i].z),
-                                      dense_residual(v[i].w));
+          for (int i = 0; i < BATCH; ++i) v[i] = src[(j + i) * STEP];
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i)
+            dst[(j + i) * STEP] = make_float4(dense_residual(v[i].x), dense_residual(v[i].y), dense_residual(v[i].z),
+                                              dense_residual(v[i].w));
+        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) arrive_leader(&lo_ready[l]);

@@ -253,13 +253,16 @@ MmPlan plan_mm(int64_t m, int64_t n, int64_t k, int sms) {
     int bn, g;
     double step;
   };
-  constexpr Tile kF32[] = {{64, 1, 1050}, {128, 1, 1570}, {128, 2, 1200}};
+  constexpr Tile kF32[] = {{64, 1, 1050}, {128, 1, 1570}, {128, 2, 1200}, {256, 2, 1900}};
   constexpr Tile k16[] = {{64, 1, 470}, {128, 1, 540}, {256, 1, 700}, {256, 2, 640}};
   MmPlan best{};
   double best_cost = 0;
   const int kb = int(ceil_div(k, BK));
-  for (int i = 0; i < (F32 ? 3 : 4); ++i) {
-    const Tile& t = F32 ? kF32[i % 3] : k16[i];
+  for (int i = 0; i < 4; ++i) {
+    const Tile& t = F32 ? kF32[i] : k16[i];
+    // The widest fp32 tile's epilogue (64 sums a lane) pays from K = 512 on: with
+    // GELU and pre, 100000 x 256 -> 512 172 us against 162, 8192 x 1024 -> 4096 291 against 372.
+    if (F32 && t.bn == 256 && k < 512) continue;
     const int64_t tiles = ceil_div(m, 128 * t.g) * ceil_div(n, t.bn);
     const int workers = sms / t.g;
     auto consider = [&](int64_t want) {
@@ -361,8 +364,9 @@ void run_mm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64_t k,
   if (plan.splits > 1) p.epi.part = static_cast<float*>(part), p.epi.ldp = round_up(n, 8);
   auto by_width = [&](auto amn, auto bmn) {
     constexpr bool A = decltype(amn)::value, B = decltype(bmn)::value;
-    constexpr int WIDE = sizeof(T) == 4 ? 128 : 256;
-    if (plan.g == 2) return launch_mm<T, A, B, WIDE, 2>(a, b, p, k, d, s);
+    if constexpr (sizeof(T) == 4)
+      if (plan.g == 2 && plan.bn == 128) return launch_mm<T, A, B, 128, 2>(a, b, p, k, d, s);
+    if (plan.g == 2) return launch_mm<T, A, B, 256, 2>(a, b, p, k, d, s);
     if (plan.bn == 64) return launch_mm<T, A, B, 64, 1>(a, b, p, k, d, s);
     if constexpr (sizeof(T) == 2)
       if (plan.bn == 256) return launch_mm<T, A, B, 256, 1>(a, b, p, k, d, s);
