@@ -18,6 +18,12 @@ import torch
 
 from . import _native
 
+# What torch.cuda.current_device, current_stream and is_current_stream_capturing
+# ask, without their wrappers (4 us of a 12 us call).
+_cuda_device = torch._C._cuda_getDevice
+_cuda_stream = torch._C._cuda_getCurrentRawStream
+_cuda_capturing = torch._C._cuda_isCurrentStreamCapturing
+
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTS = {"none": 0, "gelu": 1, "lrelu": 2, "sigmoid": 3}
 
@@ -87,6 +93,11 @@ def _param_dtype(p, dtype):
     return p.dtype
 
 
+def _like(x):
+    """A dense tensor of x's shape and type, by the quickest call."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def _act(name):
     if name not in ACTS:
         raise ValueError("act %r is not one of %s" % (name, ", ".join(ACTS)))
@@ -104,11 +115,11 @@ def _launch(entry, layout, values, device, ws_at=None):
     """Call `entry` on the device's current stream with the packed argument
     struct. With `ws_at` (the index of the workspace pointer) it may need a workspace."""
     lib = _native.lib()
-    if device != torch.cuda.current_device():
+    if device != _cuda_device():
         with torch.cuda.device(device):
             return _launch(entry, layout, values, device, ws_at)
-    stream = torch._C._cuda_getCurrentRawStream(device)
-    if ws_at is not None and not torch.cuda.is_current_stream_capturing():
+    stream = _cuda_stream(device)
+    if ws_at is not None and not _cuda_capturing():
         kept = _workspaces.get((device, stream))
         if kept is not None:
             values[ws_at], values[ws_at + 1] = kept[1], kept[2]
@@ -122,7 +133,7 @@ def _launch(entry, layout, values, device, ws_at=None):
     _native.check(getattr(lib, entry + "_workspace")(layout.pack(*values), ctypes.byref(need)))
     if need.value <= values[ws_at + 1]:
         _native.check(getattr(lib, entry)(layout.pack(*values), stream))
-    keep = need.value <= _WS_KEEP and not torch.cuda.is_current_stream_capturing()
+    keep = need.value <= _WS_KEEP and not _cuda_capturing()
     size = max(need.value, 1 << 20) if keep else need.value
     ws = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", device))
     if keep:
@@ -140,7 +151,7 @@ def layer_norm(x, scale, bias, eps=1e-6, stats=False):
     pt = _param_dtype(scale, x.dtype)
     scale, bias = _vector(scale, pt, c), _vector(bias, pt, c)
     shape = x.shape
-    y = x.new_empty(shape)
+    y = _like(x)
     if not stats:
         _launch("mx_layer_norm", _NORM, (xp, scale.data_ptr(), bias.data_ptr(), y.data_ptr(), 0, 0, rows, c, xs, c,
                                          code, _DT[pt], eps, 0), device)
@@ -165,7 +176,7 @@ def layer_norm_backward(dy, x, scale, mean, rstd, need_dx=True, need_params=True
     pt = _param_dtype(scale, x.dtype)
     scale = _vector(scale, pt, c)
     mean, rstd = _vector(mean, torch.float32, rows), _vector(rstd, torch.float32, rows)
-    dx = x.new_empty(x.shape) if need_dx else None
+    dx = _like(x) if need_dx else None
     dscale = dbias = None
     if need_params:
         dscale, dbias = torch.empty_like(scale), torch.empty_like(scale)
@@ -218,7 +229,7 @@ def dense_backward(dy, x, w, pre=None, act="none", slope=0.2, need_dx=True, need
         if pre is None or pre.shape != dy.shape:
             raise ValueError("the gradient of %s needs pre, of dy's shape" % act)
         pp, _, _, ps, pre = _rows(pre, "pre")
-    dx = x.new_empty(x.shape) if need_dx else None
+    dx = _like(x) if need_dx else None
     dw = x.new_empty((n, k)) if need_dw else None
     db = x.new_empty((n,)) if need_db else None
     _launch("mx_dense_backward", _DENSE_BACKWARD,
