@@ -358,8 +358,9 @@ int mx_channel_mean_noalloc(const float* x, int64_t npix, int32_t c, int64_t pix
  *   - outputs may not overlap inputs or each other, unless a field says so;
  *   - results are the same from call to call (no atomics in the sums);
  *   - arguments are checked before anything is launched (MX_E_INVALID).
- * Zero rows are allowed everywhere: outputs with rows are then empty, and
- * parameter gradients are zero. */
+ * Rows are fewer than 2^31 - 512 and shorter than 2^30 elements. Zero rows are
+ * allowed everywhere: outputs with rows are then empty, and parameter
+ * gradients are zero. */
 enum { MX_DT_F32 = 0, MX_DT_BF16 = 1, MX_DT_F16 = 2 };
 enum { MX_ACT_NONE = 0, MX_ACT_GELU = 1, MX_ACT_LRELU = 2, MX_ACT_SIGMOID = 3 };
 

@@ -94,7 +94,7 @@ template <class T>
 __device__ __forceinline__ void load8(const T* p, bool vec, int valid, float (&v)[8]) {
   if (vec && valid >= 8) {
 #pragma unroll
-    for (int h = 0; h < 8 / kVec<T>; ++h) raw_unpack<T, kVec<T>>(raw_load<T, kVec<T>>(p + h * kVec<T>), v + h * kVec<T>);
+    for (int h = 0; h < 8; h += kVec<T>) raw_unpack<T, kVec<T>>(raw_load<T, kVec<T>>(p + h), v + h);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < valid ? to_f(p[i]) : 0.0f;
@@ -216,7 +216,8 @@ __global__ void __launch_bounds__(256)
       for (int c = 0; c < CPW; ++c) wr[c] = raw_load_once<T, V>(wp[c] + i);
       float xv[R][V];
 #pragma unroll
-      for (int r = 0; r < R; ++r) raw_unpack<T, V>(raw_load<T, V>(x + int64_t(r < m ? r : m - 1) * x_stride + i), xv[r]);
+      for (int r = 0; r < R; ++r)
+        raw_unpack<T, V>(raw_load<T, V>(x + int64_t(r < m ? r : m - 1) * x_stride + i), xv[r]);
 #pragma unroll
       for (int c = 0; c < CPW; ++c) {
         float wv[V];
@@ -427,7 +428,8 @@ struct DenseCfg {
   static constexpr int REGS_CONTROL = 40, REGS_EPI = 96, REGS_SPLIT = 48;
   static_assert(!SPLIT_REGS || (THREADS == 768 && REGS_CONTROL + 4 * REGS_EPI + REGS_SPLIT <= 480), "register split");
   static constexpr int STAGING_BYTES = EPI_WARPS * 2048;  // 32 rows x 64 bytes each
-  static constexpr int SMEM_BYTES = 1024 + (STAGES + LO_STAGES) * STAGE_BYTES + STAGING_BYTES + 8 * (2 * STAGES + 2 * LO_STAGES + 5) + 16;
+  static constexpr int SMEM_BYTES =
+      1024 + (STAGES + LO_STAGES) * STAGE_BYTES + STAGING_BYTES + 8 * (2 * STAGES + 2 * LO_STAGES + 5) + 16;
   static_assert(SMEM_BYTES <= 232448 - 64, "shared memory per CTA");
   static_assert(TMEM_COLS <= 512, "TMEM columns");
 };

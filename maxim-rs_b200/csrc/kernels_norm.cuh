@@ -127,7 +127,8 @@ __device__ __forceinline__ void unpack_pairs(const Raw<T, V> (&q)[NV], uint64_t 
 #pragma unroll
   for (int j = 0; j < NV; ++j) raw_unpack<T, V>(q[j], f + j * V);
 #pragma unroll
-  for (int i = 0; i < kPairs<V * NV>; ++i) v[i] = f2_pack(f[2 * i], 2 * i + 1 < V * NV ? f[(2 * i + 1) % (V * NV)] : 0.0f);
+  for (int i = 0; i < kPairs<V * NV>; ++i)
+    v[i] = f2_pack(f[2 * i], 2 * i + 1 < V * NV ? f[(2 * i + 1) % (V * NV)] : 0.0f);
 }
 __device__ __forceinline__ float pair_sum(uint64_t v) {
   float a, b;
@@ -211,7 +212,8 @@ __global__ void __launch_bounds__(kNormThreads<L>) layer_norm_kernel(NormFwd p) 
     if constexpr (RING) {
       copy_wait<S - 1>();
 #pragma unroll
-      for (int j = 0; j < NV; ++j) cur[j] = raw_load<T, V>(reinterpret_cast<const T*>(&ring[(stage * NV + j) * L + lane]));
+      for (int j = 0; j < NV; ++j)
+        cur[j] = raw_load<T, V>(reinterpret_cast<const T*>(&ring[(stage * NV + j) * L + lane]));
       fill(r + S * step, stage);
       stage = stage + 1 == S ? 0 : stage + 1;
     } else if constexpr (HOLD) {

@@ -21,28 +21,37 @@ const OpsTable& table(const char* who, int dtype) {
 }
 int64_t size_of(int dtype) { return dtype == MX_DT_F32 ? 4 : 2; }
 
-void check_size(const char* who, const char* what, int64_t v, int64_t lo) {
-  if (v < lo || v >= (int64_t(1) << 31))
-    throw Error(fmt("%s: %s = %lld is outside %lld .. 2^31-1", who, what, (long long)v, (long long)lo));
+// Row lengths stay below 2^30, so that a kernel's index may step past the end;
+// rows are counted in 64 bits but are a coordinate of the tensor maps.
+void check_length(const char* who, const char* what, int64_t v) {
+  if (v < 1 || v >= (int64_t(1) << 30))
+    throw Error(fmt("%s: %s = %lld is outside 1 .. 2^30-1", who, what, (long long)v));
+}
+void check_rows(const char* who, const char* what, int64_t v) {
+  if (v < 0 || v >= (int64_t(1) << 31) - 512)
+    throw Error(fmt("%s: %s = %lld is outside 0 .. 2^31-513", who, what, (long long)v));
 }
 // A matrix argument: present, aligned to its elements, rows that do not overlap.
 void check_matrix(const char* who, const char* what, const void* p, int64_t rows, int64_t cols, int64_t stride,
                   int dtype) {
   if (rows == 0) return;
   if (!p) throw Error(fmt("%s: %s is null", who, what));
-  if (reinterpret_cast<uintptr_t>(p) % size_of(dtype)) throw Error(fmt("%s: %s is not aligned to its elements", who, what));
+  if (reinterpret_cast<uintptr_t>(p) % size_of(dtype))
+    throw Error(fmt("%s: %s is not aligned to its elements", who, what));
   if (stride < cols || stride >= (int64_t(1) << 36))
     throw Error(fmt("%s: %s has a row stride of %lld; its rows have %lld elements", who, what, (long long)stride,
                     (long long)cols));
 }
 void check_vector(const char* who, const char* what, const void* p, int dtype, bool optional) {
   if (!p && !optional) throw Error(fmt("%s: %s is null", who, what));
-  if (reinterpret_cast<uintptr_t>(p) % size_of(dtype)) throw Error(fmt("%s: %s is not aligned to its elements", who, what));
+  if (reinterpret_cast<uintptr_t>(p) % size_of(dtype))
+    throw Error(fmt("%s: %s is not aligned to its elements", who, what));
 }
 void check_workspace(const char* who, const void* p, int64_t have, int64_t need) {
   if (need == 0) return;
   if (!p || have < need)
-    throw Error(fmt("%s: the workspace has %lld bytes, %lld are needed", who, (long long)(p ? have : 0), (long long)need));
+    throw Error(
+        fmt("%s: the workspace has %lld bytes, %lld are needed", who, (long long)(p ? have : 0), (long long)need));
   if (reinterpret_cast<uintptr_t>(p) % 16) throw Error(fmt("%s: the workspace is not 16-byte aligned", who));
 }
 void check_act(const char* who, int act) {
@@ -77,7 +86,8 @@ OpsDevice device() {
   OpsDevice d;
   {
     std::lock_guard<std::mutex> lock(mu);
-    if (dev < 0 || dev >= kMaxDevices) throw Error(fmt("device %d is beyond the %d the operators track", dev, kMaxDevices));
+    if (dev < 0 || dev >= kMaxDevices)
+      throw Error(fmt("device %d is beyond the %d the operators track", dev, kMaxDevices));
     if (!sms[dev]) MX_CUDA(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev));
     d.sms = sms[dev];
   }
@@ -95,8 +105,8 @@ void check(const mx_layer_norm_args& a) {
   const char* who = "mx_layer_norm";
   table(who, a.dtype);
   check_param_dtype(who, a.dtype, a.param_dtype);
-  check_size(who, "rows", a.rows, 0);
-  check_size(who, "c", a.c, 1);
+  check_rows(who, "rows", a.rows);
+  check_length(who, "c", a.c);
   check_matrix(who, "x", a.x, a.rows, a.c, a.x_stride, a.dtype);
   check_matrix(who, "y", a.y, a.rows, a.c, a.y_stride, a.dtype);
   check_vector(who, "scale", a.scale, a.param_dtype, false);
@@ -109,8 +119,8 @@ void check(const mx_layer_norm_backward_args& a) {
   const char* who = "mx_layer_norm_backward";
   table(who, a.dtype);
   check_param_dtype(who, a.dtype, a.param_dtype);
-  check_size(who, "rows", a.rows, 0);
-  check_size(who, "c", a.c, 1);
+  check_rows(who, "rows", a.rows);
+  check_length(who, "c", a.c);
   check_matrix(who, "dy", a.dy, a.rows, a.c, a.dy_stride, a.dtype);
   check_matrix(who, "x", a.x, a.rows, a.c, a.x_stride, a.dtype);
   if (a.dx) check_matrix(who, "dx", a.dx, a.rows, a.c, a.dx_stride, a.dtype);
@@ -124,9 +134,9 @@ void check(const mx_dense_args& a) {
   const char* who = "mx_dense";
   table(who, a.dtype);
   check_act(who, a.act);
-  check_size(who, "m", a.m, 0);
-  check_size(who, "k", a.k, 1);
-  check_size(who, "n", a.n, 1);
+  check_rows(who, "m", a.m);
+  check_length(who, "k", a.k);
+  check_length(who, "n", a.n);
   check_matrix(who, "x", a.x, a.m, a.k, a.x_stride, a.dtype);
   check_matrix(who, "w", a.w, a.n, a.k, a.w_stride, a.dtype);
   check_matrix(who, "y", a.y, a.m, a.n, a.y_stride, a.dtype);
@@ -138,9 +148,9 @@ void check(const mx_dense_backward_args& a) {
   const char* who = "mx_dense_backward";
   table(who, a.dtype);
   check_act(who, a.act);
-  check_size(who, "m", a.m, 0);
-  check_size(who, "k", a.k, 1);
-  check_size(who, "n", a.n, 1);
+  check_rows(who, "m", a.m);
+  check_length(who, "k", a.k);
+  check_length(who, "n", a.n);
   check_matrix(who, "dy", a.dy, a.m, a.n, a.dy_stride, a.dtype);
   if (a.act != MX_ACT_NONE) check_matrix(who, "pre", a.pre, a.m, a.n, a.pre_stride, a.dtype);
   if (a.dx) {

@@ -121,10 +121,12 @@ void norm_forward_v(const mx_layer_norm_args& a, const OpsDevice& d, cudaStream_
   const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto nv) {
     constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
     constexpr int THREADS = kNormThreads<L>, GROUPS = THREADS / L;
-    const int64_t blocks = std::min<int64_t>(ceil_div(a.rows, GROUPS), int64_t(d.sms) * norm_resident<T, V, L, NV, false>());
+    const int64_t resident = norm_resident<T, V, L, NV, false>();
+    const int64_t blocks = std::min<int64_t>(ceil_div(a.rows, GROUPS), d.sms * resident);
     launch(layer_norm_kernel<T, V, L, NV>, dim3(unsigned(blocks)), THREADS, kNormSmem<V, L, NV, 1>, s, p);
   });
-  if (!done) launch(layer_norm_long_kernel<T, V>, dim3(unsigned(std::min<int64_t>(a.rows, int64_t(d.sms) * 4))), 512, 0, s, p);
+  if (!done)
+    launch(layer_norm_long_kernel<T, V>, dim3(unsigned(std::min<int64_t>(a.rows, int64_t(d.sms) * 4))), 512, 0, s, p);
 }
 
 template <class T>
@@ -175,9 +177,11 @@ void norm_backward_v(const mx_layer_norm_backward_args& a, const OpsDevice& d, c
   if (!done) {
     // The sums first: dx may overwrite dy.
     if (part)
-      launch(layer_norm_param_long_kernel<T, V>, dim3(unsigned(ceil_div(a.c, 32 * V)), unsigned(n.blocks)), 256, 0, s, p);
+      launch(layer_norm_param_long_kernel<T, V>, dim3(unsigned(ceil_div(a.c, 32 * V)), unsigned(n.blocks)), 256, 0, s,
+             p);
     if (a.dx)
-      launch(layer_norm_dx_long_kernel<T, V>, dim3(unsigned(std::min<int64_t>(a.rows, int64_t(d.sms) * 4))), 512, 0, s, p);
+      launch(layer_norm_dx_long_kernel<T, V>, dim3(unsigned(std::min<int64_t>(a.rows, int64_t(d.sms) * 4))), 512, 0, s,
+             p);
   }
 }
 
@@ -318,7 +322,8 @@ CUtensorMap result_map(void* p, int64_t stride, int64_t rows, int64_t cols, int6
   const cuuint32_t box[3] = {64 / sizeof(U), 32, 1}, es[3] = {1, 1, 1};
   CUtensorMap m;
   CUresult r = tensor_map_encoder()(&m, map_type<U>(), 3, p, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                    CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                    CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw Error(fmt("cuTensorMapEncodeTiled failed (%d)", int(r)), MX_E_CUDA);
   return m;
 }
@@ -384,7 +389,8 @@ void run_mm(const Operand& a, const Operand& b, int64_t m, int64_t n, int64_t k,
     if (plan.splits >= 16 && vecs < int64_t(d.sms) * 512)
       launch(dense_join_kernel<T, 8>, dim3(unsigned(ceil_div(vecs, 32))), 256, 0, s, p.epi, plan.splits, m, n);
     else
-      launch(dense_join_kernel<T, 1>, dim3(unsigned(std::min<int64_t>(ceil_div(vecs, 256), int64_t(d.sms) * 8))), 256, 0, s, p.epi, plan.splits, m, n);
+      launch(dense_join_kernel<T, 1>, dim3(unsigned(std::min<int64_t>(ceil_div(vecs, 256), int64_t(d.sms) * 8))), 256,
+             0, s, p.epi, plan.splits, m, n);
   }
 }
 
@@ -469,9 +475,9 @@ void dense_rows(const mx_dense_args& a, const DenseEpi& epi, const OpsDevice& d,
   const int warps = std::max(4, ks);
   const unsigned grid = unsigned(ceil_div(ceil_div(a.n, cpw), warps / ks));
   auto go = [&](auto r, auto v, auto c) {
-    launch(dense_rows_kernel<T, decltype(r)::value, decltype(v)::value, decltype(c)::value>, dim3(grid), warps * 32, 0, s, 
-        static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.w), a.w_stride, epi, int(a.m), int(a.n),
-        int(a.k), ks);
+    launch(dense_rows_kernel<T, decltype(r)::value, decltype(v)::value, decltype(c)::value>, dim3(grid), warps * 32, 0,
+           s, static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.w), a.w_stride, epi, int(a.m),
+           int(a.n), int(a.k), ks);
   };
   auto by_cols = [&](auto r, auto v) {
     if (cpw == 4)

@@ -219,7 +219,8 @@ ACTS = ["none", "gelu", "lrelu", "sigmoid"]
 # Few rows (the FMA kernel), one tile and less, ragged tiles, split sums, odd and unaligned sizes, depth.
 DENSE_MKN = [(1, 1, 1), (1, 4096, 1000), (2, 31, 7), (3, 520, 8000), (4, 64, 64), (5, 513, 130), (8, 1024, 333),
              (9, 64, 64), (16, 5, 3), (33, 96, 40), (128, 64, 64), (129, 65, 257), (200, 1000, 1000), (64, 8192, 128),
-             (517, 1023, 771), (1000, 128, 256), (2500, 72, 31), (300, 3000, 2049), (70000, 16, 24), (4000, 512, 1536)]
+             (517, 1023, 771), (1000, 128, 256), (2500, 72, 31), (300, 3000, 2049), (70000, 16, 24), (4000, 512, 1536),
+             (100, 300, 40000), (2048, 1032, 1100)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -395,6 +396,23 @@ def test_graph_capture(ops):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_offsets_past_32_bits(ops, dtype):
+    """A channel range of a tensor of 4.6e9 elements: the last rows lie past 2^32 of them."""
+    wide = torch.empty(70000, 65536, dtype=dtype, device="cuda")
+    x = wide[:, 60000:60096]
+    x.copy_(rand(1, 70000, 96, dtype=dtype))
+    scale, bias = rand(2, 96, scale=0.1, shift=1.0), rand(3, 96)
+    check_ln(ops, x, scale, bias)
+    _, mean, rstd = ops.layer_norm(x, scale, bias, stats=True)
+    check_ln_backward(ops, x, x, scale, mean, rstd)
+    w = rand(4, 40, 96, dtype=dtype, scale=0.1)
+    check_dense(ops, x, w, None, "gelu", rand(5, 70000, 40, dtype=dtype))
+    dy = wide[:, 50000:50040]
+    dy.copy_(rand(6, 70000, 40, dtype=dtype))
+    check_dense_backward(ops, dy, x, w, "none", None)
 
 
 def test_refusals(ops, mx):

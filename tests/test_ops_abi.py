@@ -23,7 +23,8 @@ def ops():
 
 def c_fields(name):
     text = open(os.path.join(ROOT, "include", "maxim_b200.h")).read()
-    body = re.search(r"typedef struct %s \{(.*?)\}" % name, re.sub(r"/\*.*?\*/", "", text, flags=re.S), flags=re.S).group(1)
+    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    body = re.search(r"typedef struct %s \{(.*?)\}" % name, text, flags=re.S).group(1)
     fields = []
     for line in body.split(";"):
         if not line.strip():
