@@ -257,7 +257,8 @@ __global__ void __launch_bounds__(256)
 // d = dy act'(pre) and the partial column sums of d (over fp32 values, before
 // d is rounded to the operands' type for the two products). A block takes
 // lx V columns (lx = 32, or fewer lanes where the matrix is narrow) of a range of
-// rows, 256 / lx rows at a time. With act none nothing is written but the sums.
+// rows, 256 / lx rows at a time. With act none, or d null,
+// nothing is written but the sums.
 // GELU's derivative is about 17 instructions an element, which in 16 bits is as
 // long as the memory's time.
 template <class T, int V>
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(256, 3)
           float q[V];
           raw_unpack<T, V>(pr[i], q);
           apply_act_grad<V>(act, v, q, slope);
-          if (r < m) raw_store<T, V>(d + r * d_stride + col, raw_pack<T, V>(v));
+          if (d && r < m) raw_store<T, V>(d + r * d_stride + col, raw_pack<T, V>(v));
         }
 #pragma unroll
         for (int k = 0; k < V; ++k) a[k] += v[k];

@@ -246,9 +246,9 @@ struct MmPlan {
 // splits over sizes from 64 x 512 x 512 to 20000 x 344 x 704 (the choice is within a few
 // percent of the best of each). A k-block (128 bytes of K) of a tile costs
 // `step` cycles, mostly its operands' way from the L2; a launch, its first
-// loads and last epilogue cost 7000; the CTAs of the slowest SM are what
-// counts. Split sums cost their write and reading back (2000 bytes a cycle
-// for the whole GPU) and another launch (5000).
+// loads and last epilogue cost 7000 (8700 for pairs); the CTAs of the slowest SM
+// are what counts. Split sums cost their write and reading back (3000 bytes a
+// cycle for the whole GPU) and another launch (3500).
 template <class T>
 MmPlan plan_mm(int64_t m, int64_t n, int64_t k, int sms) {
   constexpr bool F32 = sizeof(T) == 4;
@@ -258,7 +258,7 @@ MmPlan plan_mm(int64_t m, int64_t n, int64_t k, int sms) {
     double step;
   };
   constexpr Tile kF32[] = {{64, 1, 1050}, {128, 1, 1570}, {128, 2, 1200}, {256, 2, 1900}};
-  constexpr Tile k16[] = {{64, 1, 470}, {128, 1, 540}, {256, 1, 700}, {256, 2, 640}};
+  constexpr Tile k16[] = {{64, 1, 470}, {128, 1, 540}, {256, 1, 740}, {256, 2, 640}};
   MmPlan best{};
   double best_cost = 0;
   const int kb = int(ceil_div(k, BK));
@@ -273,8 +273,8 @@ MmPlan plan_mm(int64_t m, int64_t n, int64_t k, int sms) {
       if (want < 1 || want > kb || (want > 1 && tiles * want > int64_t(workers) * 2)) return;
       const int per = int(ceil_div(kb, want)), splits = int(ceil_div(kb, per));
       const int64_t waves = ceil_div(tiles * splits, workers);
-      double cost = double(waves) * (per * t.step + 1000) + 7000;
-      if (splits > 1) cost += 5000 + double(splits) * double(m) * double(n) * 8 / 2000;
+      double cost = double(waves) * (per * t.step + 1000) + (t.g == 2 ? 8700 : 7000);
+      if (splits > 1) cost += 3500 + double(splits) * double(m) * double(n) * 8 / 3000;
       if (best.bn == 0 || cost < best_cost) {
         best_cost = cost;
         best = {t.bn, t.g, splits, kb, per, splits > 1 ? int64_t(splits) * m * round_up(n, 8) * 4 : 0};
@@ -542,7 +542,7 @@ struct DenseBackward {
         x(c, a.dw ? a.x : nullptr, a.dw ? a.x_stride : 0, a.m, a.k),
         w(c, a.dx ? a.w : nullptr, a.dx ? a.w_stride : 0, a.n, a.k), dx{}, dw{}, part(nullptr) {
     vec = aligned<T>(a.dy, a.dy_stride) && (!act || aligned<T>(a.pre, a.pre_stride)) && a.n % kVec<T> == 0;
-    if (act || a.db) {
+    if ((act && products) || a.db) {
       const int64_t vecs = ceil_div(a.n, vec ? kVec<T> : 1);
       while (lx_log2 > 0 && (int64_t(1) << (lx_log2 - 1)) >= vecs) --lx_log2;
       cols = ceil_div(vecs, int64_t(1) << lx_log2);
@@ -553,7 +553,7 @@ struct DenseBackward {
       chunks = cluster ? std::min<int64_t>(8, ceil_div(a.m, 2 * subs))
                        : std::min<int64_t>(ceil_div(a.m, 2 * subs), std::max<int64_t>(1, int64_t(dev.sms) * 6 / cols));
     }
-    if (act) d = static_cast<T*>(c.take(a.m * d_stride * int64_t(sizeof(T))));
+    if (act && products) d = static_cast<T*>(c.take(a.m * d_stride * int64_t(sizeof(T))));
     if (a.db && !cluster) db_part = static_cast<float*>(c.take(chunks * a.n * 4));
     if (a.dx) dx = plan_mm<T>(a.m, a.k, a.n, dev.sms);
     if (a.dw) dw = plan_mm<T>(a.n, a.k, a.m, dev.sms);
@@ -578,7 +578,7 @@ void dense_backward(const mx_dense_backward_args& a, const OpsDevice& dev, cudaS
   }
   Carver c{static_cast<uint8_t*>(a.workspace)};
   DenseBackward<T> b(c, a, dev);
-  if (b.act || a.db) {
+  if (b.chunks) {
     auto go = [&](auto v) {
       constexpr int V = decltype(v)::value;
       launch_clusters(dense_grad_kernel<T, V>, dim3(unsigned(b.cols), unsigned(b.chunks)), dim3(256), 0,
