@@ -78,6 +78,11 @@ __device__ __forceinline__ void row_sum(float (&s)[K], float (*red)[32 * K], int
 
 template <int L>
 constexpr int kNormThreads = L <= 32 ? 256 : L;
+// Blocks an SM is asked to hold (0: the compiler's own choice of registers).
+// Asking for one lets a row's block have more of them: 20000 x 1000 fp16 backward
+// 40 to 35 us, 32768 x 2048 bf16 forward 51 to 46; the other shapes lose by it.
+template <int V, int L, bool BACKWARD>
+constexpr int kNormMinBlocks = BACKWARD ? (L == 128 || L == 512) : (V > 1 && L > 32);
 // Up to 16 values a thread the parameters and the next row fit in registers too.
 template <int V, int NV>
 constexpr bool kNormHold = V * NV <= 16;
@@ -89,9 +94,10 @@ constexpr bool kNormHold = V * NV <= 16;
 // backward.) Short rows, many to a block, have enough in flight in registers.
 template <int V, int L>
 constexpr bool kNormRing = V > 1 && L > 32;
-// Stages of `bytes` each: up to 4 in 64 KB, else 2, else 1 (the next row is
-// on its way while the current one is worked on in registers).
-constexpr int norm_stages(int bytes) { return bytes <= 16384 ? 4 : (bytes <= 65536 ? 2 : 1); }
+// Stages of `bytes` each: 3 up to 16 KB (a fourth measured 1 to 3 us slower), else
+// 2, else 1 (the next row is on its way while the current one is worked on in
+// registers).
+constexpr int norm_stages(int bytes) { return bytes <= 16384 ? 3 : (bytes <= 65536 ? 2 : 1); }
 template <int V, int L, int NV, int TENSORS>
 constexpr int kNormStages = norm_stages(L * NV * 16 * TENSORS);
 template <int V, int L, int NV, int TENSORS>
@@ -137,7 +143,7 @@ __device__ __forceinline__ float pair_sum(uint64_t v) {
 }
 
 template <class T, int V, int L, int NV>
-__global__ void __launch_bounds__(kNormThreads<L>) layer_norm_kernel(NormFwd p) {
+__global__ void __launch_bounds__(kNormThreads<L>, kNormMinBlocks<V, L, false>) layer_norm_kernel(NormFwd p) {
   sm100::pdl_wait();
   constexpr int E = V * NV, P = kPairs<E>;
   constexpr bool HOLD = kNormHold<V, NV>;
@@ -339,7 +345,7 @@ __global__ void __launch_bounds__(512) layer_norm_long_kernel(NormFwd p) {
 }
 
 template <class T, int V, int L, int NV>
-__global__ void __launch_bounds__(kNormThreads<L>) layer_norm_backward_kernel(NormBwd p) {
+__global__ void __launch_bounds__(kNormThreads<L>, kNormMinBlocks<V, L, true>) layer_norm_backward_kernel(NormBwd p) {
   sm100::pdl_wait();
   constexpr int E = V * NV, P = kPairs<E>;
   constexpr bool HOLD = kNormHold<V, NV>;

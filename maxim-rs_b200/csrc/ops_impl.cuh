@@ -57,9 +57,11 @@ void launch(void (*kernel)(P...), dim3 grid, unsigned threads, int smem, cudaStr
 // a lane); past that a warp or a block with 16 values a thread, then 32.
 // (Twice the lanes with 8 values each measured slower: 16411 x 4096 bf16
 // backward 100 us against 77, the reductions cost a warp the same.)
+// Two warps a row pay forward only (65536 x 1024 bf16: forward 55 to 48 us, backward
+// 82 to 92).
 // f(L, NV) is called with the choice as integral constants; returns false for
 // rows too long.
-template <int V, class F>
+template <int V, bool BACKWARD, class F>
 bool with_norm_shape(int c, F&& f) {
   constexpr int N8 = V < 8 ? 8 / V : 1, N16 = 16 / V;
   const int64_t vecs = ceil_div(c, V);
@@ -75,6 +77,7 @@ bool with_norm_shape(int c, F&& f) {
   MX_SHAPE(16, N8)
   MX_SHAPE(32, N8)
   MX_SHAPE(32, N16)
+  if constexpr (!BACKWARD && V > 1) MX_SHAPE(64, N16)
   MX_SHAPE(128, N8)
   MX_SHAPE(128, N16)
   MX_SHAPE(256, N16)
@@ -118,7 +121,7 @@ template <class T, int V>
 void norm_forward_v(const mx_layer_norm_args& a, const OpsDevice& d, cudaStream_t s) {
   NormFwd p{a.x, a.scale, a.bias, a.y, a.mean, a.rstd, a.rows, a.x_stride, a.y_stride,
             int(a.c), a.param_dtype == MX_DT_F32, a.eps};
-  const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto nv) {
+  const bool done = with_norm_shape<V, false>(int(a.c), [&](auto l, auto nv) {
     constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
     constexpr int THREADS = kNormThreads<L>, GROUPS = THREADS / L;
     const int64_t resident = norm_resident<T, V, L, NV, false>();
@@ -151,7 +154,7 @@ struct NormBlocks {
 template <class T, int V>
 NormBlocks norm_backward_blocks(const mx_layer_norm_backward_args& a, const OpsDevice& d) {
   NormBlocks n{0, false};
-  const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto nv) {
+  const bool done = with_norm_shape<V, true>(int(a.c), [&](auto l, auto nv) {
     constexpr int L = decltype(l)::value, NV = decltype(nv)::value, GROUPS = kNormThreads<L> / L;
     const int resident = norm_resident<T, V, L, NV, true>();
     const int64_t want = ceil_div(a.rows, GROUPS);
@@ -168,7 +171,7 @@ void norm_backward_v(const mx_layer_norm_backward_args& a, const OpsDevice& d, c
   float* part = (a.dscale || a.dbias) && !n.cluster ? static_cast<float*>(a.workspace) : nullptr;
   NormBwd p{a.dy, a.x, a.scale, a.mean, a.rstd, a.dx, part, n.cluster ? int(n.blocks) : 0, a.dscale, a.dbias,
             a.rows, a.dy_stride, a.x_stride, a.dx_stride, int(a.c), a.param_dtype == MX_DT_F32};
-  const bool done = with_norm_shape<V>(int(a.c), [&](auto l, auto nv) {
+  const bool done = with_norm_shape<V, true>(int(a.c), [&](auto l, auto nv) {
     constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
     const int smem = kNormSmem<V, L, NV, 2> + (n.cluster ? int(2 * a.c * 4) : 0);
     launch_clusters(layer_norm_backward_kernel<T, V, L, NV>, dim3(unsigned(n.blocks)), dim3(kNormThreads<L>), smem,
