@@ -7,6 +7,7 @@ roundoff: a result is rounded once to its type, U[t] |y|. Sums run in fp32:
 a sum of terms s with at most d roundings in any term's path is off by
 d 2^-23 sum |s| (2^-23, not 2^-24: the tensor cores' accumulators truncate).
 """
+import ctypes
 import importlib
 import math
 
@@ -396,6 +397,62 @@ def test_graph_capture(ops):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+def c_call(mx, ops, entry, layout, values, ws_at=None):
+    """A call through the C ABI, its workspace filled with NaN bytes."""
+    ws = None
+    if ws_at is not None:
+        need = ctypes.c_int64()
+        mx._native.check(getattr(mx.lib(), entry + "_workspace")(layout.pack(*values), ctypes.byref(need)))
+        ws = torch.full((need.value + 16,), 255, dtype=torch.uint8, device="cuda")
+        values[ws_at], values[ws_at + 1] = ws.data_ptr(), need.value
+    mx._native.check(getattr(mx.lib(), entry)(layout.pack(*values), torch.cuda.current_stream().cuda_stream))
+    return ws
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [5, 8])  # unaligned and aligned rows of the outputs
+def test_strided_outputs_and_in_place_results(mx, ops, dtype, gap):
+    """The C ABI's output strides: what lies between the rows stays, at every size; and results over their inputs."""
+    code = ops._DT[dtype]
+    for m, k, n in ((1, 64, 48), (40, 72, 48), (300, 200, 136), (700, 1000, 264), (64, 4096, 64)):
+        x, w = rand(1, m, k, dtype=dtype), rand(2, n, k, dtype=dtype, scale=1 / math.sqrt(k))
+        res, dy = rand(3, m, n, dtype=dtype), rand(4, m, n, dtype=dtype)
+        want, want_pre = ops.dense(x, w, act="gelu", residual=res, save_pre=True)
+        y, pre = (torch.full((m, n + gap), 7.0, dtype=dtype, device="cuda") for _ in range(2))
+        y[:, :n] = res  # the residual's place becomes the result's
+        P = torch.Tensor.data_ptr
+        keep = c_call(mx, ops, "mx_dense", ops._DENSE, [P(x), P(w), 0, P(y), P(y), P(pre), 0, 0, m, k, n, k, k, n + gap,
+                                                        n + gap, n + gap, code, 1, 0.0, 0], 6)
+        assert torch.equal(y[:, :n], want) and torch.equal(pre[:, :n], want_pre), (m, k, n)
+        assert (y[:, n:] == 7).all() and (pre[:, n:] == 7).all()
+        dx, dw = (torch.full((r, k + gap), 7.0, dtype=dtype, device="cuda") for r in (m, n))
+        db = torch.empty(n, dtype=dtype, device="cuda")
+        keep2 = c_call(mx, ops, "mx_dense_backward", ops._DENSE_BACKWARD,
+                       [P(dy), P(x), P(w), P(want_pre), P(dx), P(dw), P(db), 0, 0, m, k, n, n, k, k, n, k + gap, k + gap,
+                        code, 1, 0.0, 0], 7)
+        got = ops.dense_backward(dy, x, w, pre=want_pre, act="gelu")
+        assert all(torch.equal(a, b) for a, b in zip((dx[:, :k], dw[:, :k], db), got)), (m, k, n)
+        assert (dx[:, k:] == 7).all() and (dw[:, k:] == 7).all()
+        scale, bias = rand(5, k, shift=1.0), rand(6, k)
+        want, mean, rstd = ops.layer_norm(x, scale, bias, stats=True)
+        z = torch.full((m, k + gap), 7.0, dtype=dtype, device="cuda")
+        z[:, :k] = x
+        c_call(mx, ops, "mx_layer_norm", ops._NORM,
+               [P(z), P(scale), P(bias), P(z), 0, 0, m, k, k + gap, k + gap, code, 0, 1e-6, 0])
+        # Unaligned rows are summed in another order.
+        close(z[:, :k], want.double(), 1e-5 * (1 + want.double().abs()) + 2 * U[dtype] * want.double().abs(), "in place")
+        assert (z[:, k:] == 7).all()
+        g = rand(7, m, k, dtype=dtype)
+        want = ops.layer_norm_backward(g, x, scale, mean, rstd)[0]
+        z[:, :k] = g
+        c_call(mx, ops, "mx_layer_norm_backward", ops._NORM_BACKWARD,
+               [P(z), P(x), P(scale), P(mean), P(rstd), P(z), 0, 0, 0, 0, m, k, k + gap, k, k + gap, code, 0], 8)
+        close(z[:, :k], want.double(), 1e-5 * (1 + want.double().abs()) + 2 * U[dtype] * want.double().abs(), "in place")
+        assert (z[:, k:] == 7).all()
+        torch.cuda.synchronize()
+        del keep, keep2
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
