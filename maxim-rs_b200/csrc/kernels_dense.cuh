@@ -257,10 +257,11 @@ __global__ void __launch_bounds__(256)
 // d = dy act'(pre) and the partial column sums of d (over fp32 values, before
 // d is rounded to the operands' type for the two products). A block takes
 // lx V columns (lx = 32, or fewer lanes where the matrix is narrow) of a range of
-// rows, 256 / lx rows at a time. With act none, or d null,
-// nothing is written but the sums.
-// GELU's derivative is about 17 instructions an element, which in 16 bits is as
-// long as the memory's time.
+// rows, 256 / lx rows at a time. With act none, or d null, nothing is written but
+// the sums. GELU's derivative is about 17 instructions an element, which in 16
+// bits is as long as the memory's time. With an activation, what is read here
+// leaves the L2 first, so that more of d is still there for the products
+// (gradient of 71680 x 128 -> 256 fp32: 105 us to 101).
 template <class T, int V>
 __global__ void __launch_bounds__(256, 3)
     dense_grad_kernel(const T* dy, int64_t dy_stride, const T* pre, int64_t pre_stride, T* d, int64_t d_stride,
@@ -283,8 +284,12 @@ __global__ void __launch_bounds__(256, 3)
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
         const int64_t r = r0 + i * step;
-        dr[i] = r < m ? raw_load<T, V>(dy + r * dy_stride + col) : raw_zero<T, V>();
-        if (act != MX_ACT_NONE) pr[i] = r < m ? raw_load<T, V>(pre + r * pre_stride + col) : raw_zero<T, V>();
+        if (act == MX_ACT_NONE) {
+          dr[i] = r < m ? raw_load<T, V>(dy + r * dy_stride + col) : raw_zero<T, V>();
+        } else {
+          dr[i] = r < m ? raw_load_streaming<T, V>(dy + r * dy_stride + col) : raw_zero<T, V>();
+          pr[i] = r < m ? raw_load_streaming<T, V>(pre + r * pre_stride + col) : raw_zero<T, V>();
+        }
       }
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {

@@ -70,6 +70,17 @@ __device__ __forceinline__ Raw<T, V> raw_load_once(const T* p) {
   }
   return r;
 }
+// Data that is read once, first to leave the L2.
+template <class T, int V>
+__device__ __forceinline__ Raw<T, V> raw_load_streaming(const T* p) {
+  Raw<T, V> r;
+  if constexpr (V == 1) {
+    r.u = *p;
+  } else {
+    r.u = __ldcs(reinterpret_cast<const uint4*>(p));
+  }
+  return r;
+}
 template <class T, int V>
 __device__ __forceinline__ Raw<T, V> raw_zero() {
   Raw<T, V> r;
