@@ -13,6 +13,7 @@ transpose, an expanded gradient) is copied first.
 """
 import ctypes
 import struct
+import threading
 
 import torch
 
@@ -104,11 +105,21 @@ def _act(name):
     return ACTS[name]
 
 
-# Workspaces up to _WS_KEEP bytes stay with their stream: its calls run one
-# after the other, so they can share one. Larger ones, and those of a captured
-# graph (which must own its memory), come from torch's allocator at each call.
+# Workspaces up to _WS_KEEP bytes stay with the host thread and stream that they
+# were made for. Not with the stream alone: a call issues several kernels that
+# hand data on through its workspace, and does so without the interpreter's
+# lock, so the kernels of two threads' calls may lie in a stream in any order.
+# Larger ones, and those of a captured graph (which must own its memory), come
+# from torch's allocator at each call.
 _WS_KEEP = 32 << 20
-_workspaces = {}
+
+
+class _Kept(threading.local):
+    def __init__(self):
+        self.by_stream = {}  # (device, stream): (tensor, address, bytes)
+
+
+_kept = _Kept()
 
 
 def _launch(entry, layout, values, device, ws_at=None):
@@ -119,25 +130,28 @@ def _launch(entry, layout, values, device, ws_at=None):
         with torch.cuda.device(device):
             return _launch(entry, layout, values, device, ws_at)
     stream = _cuda_stream(device)
-    if ws_at is not None and not _cuda_capturing():
-        kept = _workspaces.get((device, stream))
-        if kept is not None:
-            values[ws_at], values[ws_at + 1] = kept[1], kept[2]
+    if ws_at is None:
+        return _native.check(getattr(lib, entry)(layout.pack(*values), stream))
+    capturing = _cuda_capturing()
+    # Held until the kernels are issued: from then on the stream's order protects it.
+    kept = None if capturing else _kept.by_stream.get((device, stream))
+    if kept is not None:
+        values[ws_at], values[ws_at + 1] = kept[1], kept[2]
     rc = getattr(lib, entry)(layout.pack(*values), stream)
     if rc == _native.MX_OK:
         return
-    if rc != _native.MX_E_INVALID or ws_at is None:
+    if rc != _native.MX_E_INVALID:
         _native.check(rc)
     # Refused, perhaps only for the workspace: the query refuses too if not.
     need = ctypes.c_int64()
     _native.check(getattr(lib, entry + "_workspace")(layout.pack(*values), ctypes.byref(need)))
     if need.value <= values[ws_at + 1]:
-        _native.check(getattr(lib, entry)(layout.pack(*values), stream))
-    keep = need.value <= _WS_KEEP and not _cuda_capturing()
+        _native.check(rc)
+    keep = need.value <= _WS_KEEP and not capturing
     size = max(need.value, 1 << 20) if keep else need.value
     ws = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", device))
     if keep:
-        _workspaces[device, stream] = (ws, ws.data_ptr(), size)
+        _kept.by_stream[device, stream] = (ws, ws.data_ptr(), size)
     values[ws_at], values[ws_at + 1] = ws.data_ptr(), size
     _native.check(getattr(lib, entry)(layout.pack(*values), stream))
 

@@ -10,6 +10,7 @@ d 2^-23 sum |s| (2^-23, not 2^-24: the tensor cores' accumulators truncate).
 import ctypes
 import importlib
 import math
+import threading
 
 import pytest
 import torch
@@ -382,6 +383,72 @@ def test_other_streams(ops):
             outs.append(ops.dense(x, w, act="gelu"))
     s.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+def overlapping_calls(ops):
+    """Calls that hand data on through their workspace: unaligned copies, split sums, the activation's gradient."""
+    def forward(seed, m, k, n):
+        x, w = rand(seed, m, k, dtype=BF16), rand(seed + 1, n, k, dtype=BF16, scale=0.03)
+        return lambda: (ops.dense(x, w, act="gelu"),)
+
+    def backward(seed, m, k, n):
+        x, w = rand(seed, m, k, dtype=BF16), rand(seed + 1, n, k, dtype=BF16, scale=0.03)
+        dy, pre = rand(seed + 2, m, n, dtype=BF16), rand(seed + 3, m, n, dtype=BF16)
+        return lambda: ops.dense_backward(dy, x, w, pre=pre, act="gelu")
+
+    def norm(seed, rows, c):
+        x, dy = rand(seed, rows, c), rand(seed + 1, rows, c)
+        _, mean, rstd = ops.layer_norm(x, dy[0], dy[1], stats=True)
+        return lambda: ops.layer_norm_backward(dy, x, dy[0], mean, rstd)
+
+    return [forward(1, 300, 1023, 900), backward(11, 700, 512, 1000), norm(21, 3000, 257), forward(31, 64, 8192, 128),
+            backward(41, 90, 333, 77), backward(51, 2500, 256, 264)]
+
+
+def test_threads_on_one_stream(ops):
+    """Host threads that call on the same stream at once get what serial calls give."""
+    calls = overlapping_calls(ops)
+    want = [[t.clone() for t in c()] for c in calls]
+    torch.cuda.synchronize()
+    got, errors = [[] for _ in calls], []
+    start = threading.Barrier(len(calls))
+
+    def work(i):
+        try:
+            start.wait()
+            for _ in range(40):
+                got[i].append(calls[i]())
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for i, results in enumerate(got):
+        assert len(results) == 40
+        for r in results:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i])), i
+
+
+def test_streams_in_flight_together(ops):
+    """Calls issued in turn on several streams, all of them at work at the same time."""
+    calls = overlapping_calls(ops)
+    want = [[t.clone() for t in c()] for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[] for _ in calls]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(calls[i]())
+    torch.cuda.synchronize()
+    for i, results in enumerate(got):
+        for r in results:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i])), i
 
 
 def test_graph_capture(ops):
