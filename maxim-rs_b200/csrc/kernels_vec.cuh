@@ -57,14 +57,17 @@ __device__ __forceinline__ Raw<T, V> raw_load(const T* p) {
   return r;
 }
 // The same for data that is read once: kept out of the L1, fetched into the L2
-// by 256 bytes (a token's 134 MB of weights: 26.9 to 25.8 us).
+// by 256 bytes (a token's 134 MB of weights: 26.9 to 25.8 us). Not by the
+// read-only path (.nc): that wants memory which nothing writes while the kernel
+// lives, and a kernel whose blocks are set up early lives beside the one before
+// it, which may be what writes the weights. Volatile, so that it stays after pdl_wait.
 template <class T, int V>
 __device__ __forceinline__ Raw<T, V> raw_load_once(const T* p) {
   Raw<T, V> r;
   if constexpr (V == 1) {
     r.u = *p;
   } else {
-    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r.u.x), "=r"(r.u.y), "=r"(r.u.z), "=r"(r.u.w)
                  : "l"(p));
   }

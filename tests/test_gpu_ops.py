@@ -451,6 +451,31 @@ def test_streams_in_flight_together(ops):
             assert all(torch.equal(a, b) for a, b in zip(r, want[i])), i
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_calls_read_what_the_call_before_wrote(ops, dtype):
+    """Weights that the call just before made (its blocks may still be leaving) serve
+    one token and several, over and over."""
+    x, dy = rand(1, 64, 256, dtype=dtype), rand(2, 64, 512, dtype=dtype)
+    token, few = rand(3, 1, 256, dtype=dtype), rand(4, 40, 256, dtype=dtype)
+    signs = [1.0, -2.0, 0.5, -1.0]
+    grads = [(dy * s).contiguous() for s in signs]
+    want = []
+    for g in grads:
+        _, dw, _ = ops.dense_backward(g, x, x[:1].expand(512, 256).contiguous(), need_dx=False)
+        torch.cuda.synchronize()
+        want.append((ops.dense(token, dw), ops.dense(few, dw)))
+        torch.cuda.synchronize()
+    w = x[:1].expand(512, 256).contiguous()
+    got = []
+    for _ in range(50):
+        for g in grads:
+            _, dw, _ = ops.dense_backward(g, x, w, need_dx=False)  # the allocator gives the same place again
+            got.append((ops.dense(token, dw), ops.dense(few, dw)))
+            del dw
+    for i, r in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(r, want[i % 4])), i
+
+
 def test_graph_capture(ops):
     """The calls can be captured (they allocate through torch's graph pool only)."""
     x, w = rand(1, 300, 1023, dtype=BF16), rand(2, 900, 1023, dtype=BF16, scale=0.03)
