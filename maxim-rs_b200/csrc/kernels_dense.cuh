@@ -13,6 +13,7 @@
 
 #include <type_traits>
 
+#include "drain.h"
 #include "gpu_common.cuh"
 #include "kernels_vec.cuh"
 #include "sm100.cuh"
@@ -391,8 +392,9 @@ __global__ void __launch_bounds__(256) dense_align_kernel(const __grid_constant_
 // (the weights' gradient over 71,680 rows was off by 2.8e-6 of its size with
 // 1,900 rows to a set, by 6.9e-7 with 256).
 // Every wait is bounded in time; one that runs out records a code in the
-// status word, and the kernel drains its copies and MMAs, frees its TMEM and
-// returns.
+// status word and raises the abort flag of both CTAs, on which the other roles
+// stop. The kernel then lets its MMAs end and its copies land, by waits that the
+// flag does not cut short (only their own limit does), frees its TMEM and returns.
 struct DenseMm {
   int64_t m, n;
   int kb;          // k-blocks
@@ -403,7 +405,7 @@ struct DenseMm {
   int* status;
 };
 
-enum : int { kDenseErrProducer = 0x201, kDenseErrSplit, kDenseErrMmaAcc, kDenseErrMmaStage, kDenseErrEpilogue };
+enum : int { kDenseErrProducer = 0x201, kDenseErrSplit, kDenseErrMmaAcc, kDenseErrMmaStage, kDenseErrEpilogue, kDenseErrDrain };
 
 template <class T, int BN, int G>
 struct DenseCfg {
@@ -587,7 +589,11 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
   uint64_t* drained = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   __shared__ int abort_flag;
+  __shared__ uint32_t issued;  // stages that this CTA's producer has loaded
   const volatile int* vabort = &abort_flag;
+  // 16-bit pair: both CTAs' bytes count on the leader's barrier, which the MMA
+  // issuer waits on. In fp32 each CTA's split warps wait on their own.
+  constexpr bool SHARED = G == 2 && !C::F32;
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int tiles = p.tiles_m * p.tiles_n;
   const int items = tiles * p.splits;
@@ -629,7 +635,8 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
   const uint32_t tmem = *tmem_slot;
   auto fail = [&](int code) {
     *static_cast<volatile int*>(p.status) = code;  // host memory: a plain store
-    abort_flag = 1;
+    *const_cast<volatile int*>(vabort) = 1;
+    if constexpr (G == 2) cluster_st_flag(map_rank(&abort_flag, rank ^ 1), 1);
   };
   auto kb_range = [&](int split, int& k0, int& k1) {
     k0 = split * p.kb_split;
@@ -667,10 +674,6 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
             }
             uint8_t* a = base + s * C::STAGE_BYTES;
             uint8_t* b = a + C::A_BYTES;
-            // 16-bit pair: both CTAs' bytes count on the leader's barrier, which
-            // the MMA issuer waits on. In fp32 each CTA's split warps wait on
-            // their own.
-            constexpr bool SHARED = G == 2 && !C::F32;
             if (!SHARED || rank == 0) mbar_arrive_expect_tx(&full[s], (SHARED ? 2 : 1) * (C::A_BYTES + C::B_BYTES));
             const uint32_t leader_full = SHARED ? map_rank(&full[s], 0) : 0;
             auto load = [&](uint8_t* dst, const CUtensorMap* map, int c0, int c1) {
@@ -695,9 +698,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
             }
           }
         }
-        if (*vabort)  // copies in flight land before the CTA may leave
-          for (uint32_t j = it < C::STAGES ? 0 : it - C::STAGES; j < it; ++j)
-            if ((G == 2 && !C::F32 && rank != 0) || !wait(&full[j % C::STAGES], (j / C::STAGES) & 1)) break;
+        issued = it;
       }
     } else if (warp == 1) {
       // The whole warp runs the loop, so that what the MMAs take is the same in
@@ -782,11 +783,10 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
             if (C::F32 && ++l == C::LO_STAGES) l = 0, lph ^= 1;
           }
         }
-        if (!ok) {
-          if (elect_one()) commit(drained);
-          __syncwarp();
-          wait(drained, 0);
-        }
+        // No MMA is in flight past here, whether or not an epilogue still waits for it.
+        if (elect_one()) commit(drained);
+        __syncwarp();
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(drained, 0, nullptr)) && lane == 0) fail(kDenseErrDrain);
       }
     }
   } else if (warp < C::SPLIT_WARP0) {
@@ -901,6 +901,19 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
   __syncthreads();
   if constexpr (G == 2) cluster_sync_all();  // neither leaves while the other's MMAs, copies or arrivals need it
   tc_fence_after();
+  if (*vabort) {  // the same in both CTAs: whoever raised it did so before the barrier
+    if (threadIdx.x == 0 && !(SHARED && rank != 0)) {
+      uint32_t peers = issued;
+      if constexpr (SHARED) peers = cluster_ld_u32(map_rank(&issued, 1));
+      land_copies(
+          issued, peers, C::STAGES,
+          [&](uint32_t s) { mbar_arrive_expect_tx(&full[s], C::A_BYTES + C::B_BYTES); },
+          [&](uint32_t s) { mbar_complete_tx(&full[s], C::A_BYTES + C::B_BYTES); },
+          [&](uint32_t s, uint32_t parity) { return mbar_wait(&full[s], parity, nullptr); });
+    }
+    __syncthreads();
+    if constexpr (G == 2) cluster_sync_all();
+  }
   if (warp == 2) {
     if constexpr (G == 2)
       tmem_dealloc_pair(tmem, C::TMEM_COLS);

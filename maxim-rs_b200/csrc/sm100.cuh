@@ -67,6 +67,10 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// Bytes of a phase that no copy will bring.
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 // Wait for the phase with the given parity to complete. Returns false when
 // the time limit passes or when `abort` (a shared flag another role sets on
 // its own failure) becomes nonzero, so no role waits on a pipeline that has
@@ -102,6 +106,15 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
+}
+__device__ __forceinline__ uint32_t cluster_ld_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+// For a flag that other threads poll.
+__device__ __forceinline__ void cluster_st_flag(uint32_t addr, uint32_t v) {
+  asm volatile("st.relaxed.cluster.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ float cluster_ld(uint32_t addr) {
   float v;
