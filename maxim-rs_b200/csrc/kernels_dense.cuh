@@ -642,12 +642,14 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
     k0 = split * p.kb_split;
     k1 = min(p.kb, k0 + p.kb_split);
   };
+  // For what this CTA's threads and copies have written; for what the pair's have
+  // written or read; for accumulators, whose order tcgen05's fences keep.
   auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, vabort); };
-  auto arrive_leader = [&](uint64_t* bar) {
-    if constexpr (G == 2)
-      mbar_arrive_cluster(map_rank(bar, 0));
-    else
-      mbar_arrive(bar);
+  auto wait_pair = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait<G == 2 ? See::PAIR : See::CTA>(bar, parity, vabort);
+  };
+  auto wait_order = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait<G == 2 ? See::ORDER : See::CTA>(bar, parity, vabort);
   };
   auto commit = [&](uint64_t* bar) {
     if constexpr (G == 2)
@@ -668,7 +670,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
           const int row = (tm * G + rank) * 128, col = tn * BN + rank * C::BROWS;
           for (int kb = k0; kb < k1; ++kb, ++it) {
             const int s = it % C::STAGES;
-            if (!wait(&empty[s], ((it / C::STAGES) & 1) ^ 1)) {
+            if (!wait_pair(&empty[s], ((it / C::STAGES) & 1) ^ 1)) {
               fail(kDenseErrProducer);
               break;
             }
@@ -741,7 +743,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
             const bool fresh = left == 0;
             if (fresh) {
               const uint32_t acc = tc & 1;
-              ok = __all_sync(0xFFFFFFFFu, wait(&acc_empty[acc], ((tc >> 1) & 1) ^ 1));
+              ok = __all_sync(0xFFFFFFFFu, wait_order(&acc_empty[acc], ((tc >> 1) & 1) ^ 1));
               if (!ok) {
                 if (lane == 0) fail(kDenseErrMmaAcc);
                 break;
@@ -749,11 +751,12 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
               d = tmem + acc * C::SET_COLS;
               left = min(C::CHUNK, k1 - kb);
             }
-            ok = __all_sync(0xFFFFFFFFu, C::F32 ? wait(&lo_ready[l], lph) : wait(&full[s], ph));
+            ok = __all_sync(0xFFFFFFFFu, C::F32 ? wait_pair(&lo_ready[l], lph) : wait_pair(&full[s], ph));
             if (!ok) {
               if (lane == 0) fail(kDenseErrMmaStage);
               break;
             }
+            if constexpr (C::F32 && G == 2) fence_async_acquire_cluster();
             tc_fence_after();
             const uint32_t a = base_u + s * C::STAGE_BYTES, b = a + C::A_BYTES;
             const uint64_t da = desc(a, A_MN), db = desc(b, B_MN);
@@ -804,7 +807,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
       const int64_t col0 = int64_t(tn) * BN + part * C::EPI_COLS;
       // The warp decides as one: the TMEM loads below need all its lanes.
       auto take = [&] {
-        const bool got = __all_sync(0xFFFFFFFFu, wait(&acc_full[tc & 1], (tc >> 1) & 1));
+        const bool got = __all_sync(0xFFFFFFFFu, wait_order(&acc_full[tc & 1], (tc >> 1) & 1));
         if (!got && lane == 0) fail(kDenseErrEpilogue);
         tc_fence_after();
         return got;
@@ -812,7 +815,12 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
       auto give = [&] {  // the set is read: the next products may have it
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_leader(&acc_empty[tc & 1]);
+        if (lane == 0) {
+          if constexpr (G == 2)
+            mbar_arrive_cluster(map_rank(&acc_empty[tc & 1], 0));
+          else
+            mbar_arrive(&acc_empty[tc & 1]);
+        }
         ++tc;
       };
       if constexpr (C::F32) {
@@ -868,7 +876,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
       int k0, k1;
       kb_range(w / tiles, k0, k1);
       for (int kb = k0; kb < k1; ++kb) {
-        ok = __all_sync(0xFFFFFFFFu, wait(&full[s], ph) && wait(&lo_empty[l], lph ^ 1));
+        ok = __all_sync(0xFFFFFFFFu, wait(&full[s], ph) && wait_pair(&lo_empty[l], lph ^ 1));
         if (!ok) {
           if (lane == 0) fail(kDenseErrSplit);
           break;
@@ -891,7 +899,14 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) arrive_leader(&lo_ready[l]);
+        if (lane == 0) {
+          if constexpr (G == 2) {
+            fence_async_release_cluster();
+            mbar_arrive_cluster(map_rank(&lo_ready[l], 0));
+          } else {
+            mbar_arrive(&lo_ready[l]);
+          }
+        }
         if (++s == C::STAGES) s = 0, ph ^= 1;
         if (++l == C::LO_STAGES) l = 0, lph ^= 1;
       }
@@ -909,7 +924,9 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
           issued, peers, C::STAGES,
           [&](uint32_t s) { mbar_arrive_expect_tx(&full[s], C::A_BYTES + C::B_BYTES); },
           [&](uint32_t s) { mbar_complete_tx(&full[s], C::A_BYTES + C::B_BYTES); },
-          [&](uint32_t s, uint32_t parity) { return mbar_wait(&full[s], parity, nullptr); });
+          [&](uint32_t s, uint32_t parity) {
+            return mbar_wait<SHARED ? See::PAIR : See::CTA>(&full[s], parity, nullptr);
+          });
     }
     __syncthreads();
     if constexpr (G == 2) cluster_sync_all();

@@ -56,15 +56,38 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t by
 // warp then takes almost no issue slots from the working warps of its
 // sub-partition. The bounded wait below still checks its time limit.
 constexpr uint32_t kSuspendNs = 1000000;  // 1 ms
+// What a wait learns. CTA: all that this CTA's threads, or its copies, did before
+// they arrived. PAIR: the same of another CTA of the cluster. ORDER: only that
+// the phase has ended, over the cluster; enough for tensor memory, whose accesses
+// tcgen05's commit and fences order.
+enum class See { CTA, PAIR, ORDER };
+template <See SEE = See::CTA>
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendNs)
-      : "memory");
+  if constexpr (SEE == See::PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendNs)
+        : "memory");
+  else if constexpr (SEE == See::ORDER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendNs)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendNs)
+        : "memory");
   return ok != 0;
 }
 // Bytes of a phase that no copy will bring.
@@ -75,11 +98,12 @@ __device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) 
 // the time limit passes or when `abort` (a shared flag another role sets on
 // its own failure) becomes nonzero, so no role waits on a pipeline that has
 // already given up.
+template <See SEE = See::CTA>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const volatile int* abort) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (mbar_try_wait<SEE>(bar, parity)) return true;
   const uint64_t t0 = global_ns();
   for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_try_wait<SEE>(bar, parity)) return true;
     if ((i & 3) == 0) {
       if (abort && *abort) return false;
       if (global_ns() - t0 > kWaitLimitNs) return false;
@@ -125,13 +149,20 @@ __device__ __forceinline__ float cluster_ld(uint32_t addr) {
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Arrive on a barrier of the pair. The default semantics suffice for what
-// passes between the CTAs here - TMEM columns read (ordered by the tcgen05
-// fences) and operand tiles written to the arriving CTA's own shared memory
-// (made visible by the proxy fence before); a cluster-scope release here cost
-// the arriving warp about a thousand cycles.
+// Arrive on a barrier of another CTA of the cluster. By itself it orders only
+// tensor-memory accesses before a tc_fence_before (waited for with See::ORDER).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// Shared memory written by this CTA's threads, for the async proxy of another
+// CTA's instructions: the one fence before mbar_arrive_cluster, the other after
+// the wait. Restricted to shared memory: an arrival with release semantics over
+// the cluster waits for all memory, about a thousand cycles.
+__device__ __forceinline__ void fence_async_release_cluster() {
+  asm volatile("fence.proxy.async::generic.release.sync_restrict::shared::cta.cluster;" ::: "memory");
+}
+__device__ __forceinline__ void fence_async_acquire_cluster() {
+  asm volatile("fence.proxy.async::generic.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
 }
 
 // ------------------------------------------------------------------- TMA

@@ -92,6 +92,6 @@ def test_every_copy_has_landed(tmp_path):
 def test_the_flag_does_not_cut_the_drain_short():
     """The waits of the drain take no abort flag: it is up by then, and would end them at once."""
     text = open(os.path.join(CSRC, "kernels_dense.cuh")).read()
-    assert re.search(r"mbar_wait\(drained, 0, nullptr\)", text)
-    assert re.search(r"mbar_wait\(&full\[s\], parity, nullptr\)", text)
-    assert not re.search(r"[^_]wait\(drained", text)
+    drains = re.findall(r"mbar_wait(?:<[^;]*?>)?\((?:drained|&full\[s\]),[^;]*?;", text)
+    assert len(drains) == 2 and all("nullptr" in d for d in drains), drains
+    assert not re.search(r"\bwait(_pair|_order)?\(drained", text)
