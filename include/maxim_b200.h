@@ -346,7 +346,7 @@ int mx_channel_mean_noalloc(const float* x, int64_t npix, int32_t c, int64_t pix
  *   - elements are fp32, bf16 or fp16 (MX_DT_*); all sums and statistics are
  *     held in fp32, and a result is rounded once, as it is stored;
  *   - `stream` is a cudaStream_t (null: the legacy default stream); calls are
- *     asynchronous on it, allocate nothing (but for 4 bytes of page-locked
+ *     asynchronous on it, allocate nothing (but for 256 bytes of page-locked
  *     host memory at a process's first call, which must come before any
  *     stream capture), and run on the calling thread's current device, which
  *     must be able to read the pointers;
@@ -459,10 +459,18 @@ int mx_dense_backward_workspace(const mx_dense_backward_args* a, int64_t* bytes)
 int mx_dense_backward(const mx_dense_backward_args* a, void* stream);
 
 /* Whether a dense kernel finished so far has given up a wait inside its
- * pipeline (its output is then not to be used): MX_E_DEVICE, and the record is
- * cleared, else MX_OK. Does not wait for any stream; mx_dense and
- * mx_dense_backward refuse with the same status while a record stands. */
+ * pipeline (its output is then not to be used): MX_E_DEVICE, with the device in
+ * the message, else MX_OK. Does not wait for any stream. A record is kept by
+ * device and for every host thread: a thread's call of mx_dense or
+ * mx_dense_backward on that device is refused with the same status until that
+ * thread has polled, and its poll clears the record for itself alone. (A thread
+ * that makes its first call later is not told of records that others have seen.) */
 int mx_dense_poll(void);
+/* Leave such a record on the current device, to try a program's handling of it:
+ * one thread on `stream` waits for what nothing brings and gives up after
+ * limit_us (0 to 1000000; a few milliseconds at least) as a dense kernel would.
+ * Nothing else happens. */
+int mx_dense_wait_check(int64_t limit_us, void* stream);
 
 /* ------------------------------------------------------ the batch runner
  * Independent images sharded round-robin over GPUs: one worker thread and

@@ -145,6 +145,7 @@ _SIGS = {
     "mx_dense_backward_workspace": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]),
     "mx_dense_backward": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
     "mx_dense_poll": (ctypes.c_int, []),
+    "mx_dense_wait_check": (ctypes.c_int, [ctypes.c_int64, ctypes.c_void_p]),
     "mx_gpu_new_budget": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(mx_plan), ctypes.c_int64,
                                          ctypes.POINTER(ctypes.c_void_p)]),
     "mx_batch_new": (ctypes.c_int, [ctypes.POINTER(mx_batch_config), ctypes.POINTER(ctypes.c_int32), ctypes.c_int32,

@@ -2,11 +2,14 @@
 // (include/maxim_b200.h): argument checks and dispatch on the element type.
 #include "ops.h"
 
+#include <cstring>
 #include <mutex>
 #include <string>
 
 #include "common.h"
 #include "gpu_common.cuh"
+#include "sm100.cuh"
+#include "wait_record.h"
 
 namespace mx {
 namespace {
@@ -62,23 +65,29 @@ void check_param_dtype(const char* who, int dtype, int param) {
     throw Error(fmt("%s: param_dtype %d is neither the tensors' dtype nor MX_DT_F32", who, param));
 }
 
-// The status word of the dense kernels: one int of page-locked host memory
-// that every device can write, so the host reads it without a copy.
-int* g_status_host = nullptr;
-int* status_word() {
+// The status words of the dense kernels, one a device, in page-locked host
+// memory that every device can write, so the host reads them without a copy.
+struct Status {
+  int* words;
+  WaitRecords records;
+  explicit Status(int* w) : words(w), records(w) {}
+};
+Status& status() {
   static std::mutex mu;
+  static Status* made = nullptr;  // for the life of the process: kernels write it
   std::lock_guard<std::mutex> lock(mu);
-  if (!g_status_host) {
+  if (!made) {
     void* p = nullptr;
-    MX_CUDA(cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
-    *static_cast<int*>(p) = 0;
-    g_status_host = static_cast<int*>(p);
+    constexpr size_t bytes = WaitRecords::kDevices * sizeof(int);
+    MX_CUDA(cudaHostAlloc(&p, bytes, cudaHostAllocPortable | cudaHostAllocMapped));
+    std::memset(p, 0, bytes);
+    made = new Status(static_cast<int*>(p));
   }
-  return g_status_host;
+  return *made;
 }
 
 OpsDevice device() {
-  constexpr int kMaxDevices = 64;
+  constexpr int kMaxDevices = WaitRecords::kDevices;
   static std::mutex mu;
   static int sms[kMaxDevices] = {};
   int dev = 0;
@@ -91,14 +100,25 @@ OpsDevice device() {
     if (!sms[dev]) MX_CUDA(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev));
     d.sms = sms[dev];
   }
-  d.status = status_word();  // unified addressing: the host pointer serves the device too
+  d.index = dev;
+  d.status = status().words + dev;  // unified addressing: the host pointer serves the device too
   return d;
 }
 
-void check_status(const char* who) {
-  const int code = *static_cast<volatile int*>(status_word());
-  if (code)
-    throw Error(fmt("%s: an earlier dense kernel gave up a wait in its pipeline (code 0x%x)", who, code), MX_E_DEVICE);
+void check_status(const char* who, const OpsDevice& d) {
+  if (const int code = status().records.pending(d.index))
+    throw Error(fmt("%s: an earlier dense kernel on device %d gave up a wait in its pipeline (code 0x%x)", who, d.index,
+                    code),
+                MX_E_DEVICE);
+}
+
+// A wait that nothing ends, for mx_dense_wait_check.
+constexpr int kErrWaitCheck = 0x2FF;
+__global__ void wait_check_kernel(int* status, uint64_t limit_ns) {
+  __shared__ uint64_t bar;
+  sm100::mbar_init(&bar, 1);
+  sm100::fence_mbar_init();
+  if (!sm100::mbar_wait(&bar, 0, nullptr, limit_ns)) *static_cast<volatile int*>(status) = kErrWaitCheck;
 }
 
 void check(const mx_layer_norm_args& a) {
@@ -211,7 +231,7 @@ extern "C" int mx_dense(const mx_dense_args* a, void* stream) {
     check(*a);
     if (a->m == 0) return;
     const OpsDevice d = device();
-    check_status("mx_dense");
+    check_status("mx_dense", d);
     const OpsTable& t = table("mx_dense", a->dtype);
     check_workspace("mx_dense", a->workspace, a->workspace_bytes, t.dense_workspace(*a, d));
     t.dense(*a, d, static_cast<cudaStream_t>(stream));
@@ -231,7 +251,7 @@ extern "C" int mx_dense_backward(const mx_dense_backward_args* a, void* stream) 
     if (!a) throw Error("mx_dense_backward: null arguments");
     check(*a);
     const OpsDevice d = device();
-    check_status("mx_dense_backward");
+    check_status("mx_dense_backward", d);
     const OpsTable& t = table("mx_dense_backward", a->dtype);
     check_workspace("mx_dense_backward", a->workspace, a->workspace_bytes, t.dense_backward_workspace(*a, d));
     t.dense_backward(*a, d, static_cast<cudaStream_t>(stream));
@@ -240,11 +260,19 @@ extern "C" int mx_dense_backward(const mx_dense_backward_args* a, void* stream) 
 
 extern "C" int mx_dense_poll(void) {
   return guard([&] {
-    volatile int* w = status_word();
-    const int code = *w;
-    if (code) {
-      *w = 0;
-      throw Error(fmt("mx_dense_poll: a dense kernel gave up a wait in its pipeline (code 0x%x)", code), MX_E_DEVICE);
-    }
+    for (int dev = 0; dev < WaitRecords::kDevices; ++dev)
+      if (const int code = status().records.take(dev))
+        throw Error(
+            fmt("mx_dense_poll: a dense kernel on device %d gave up a wait in its pipeline (code 0x%x)", dev, code),
+            MX_E_DEVICE);
+  });
+}
+
+extern "C" int mx_dense_wait_check(int64_t limit_us, void* stream) {
+  return guard([&] {
+    if (limit_us < 0 || limit_us > 1000000)
+      throw Error(fmt("mx_dense_wait_check: limit_us = %lld is outside 0 .. 1000000", (long long)limit_us));
+    wait_check_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(device().status, uint64_t(limit_us) * 1000);
+    MX_CUDA(cudaGetLastError());
   });
 }

@@ -12,8 +12,8 @@
 namespace mx {
 
 struct OpsDevice {
-  int sms;
-  int* status;  // the dense kernels' status word, as the device sees it
+  int index, sms;
+  int* status;  // the dense kernels' status word of this device, as it sees it
 };
 
 // One element type's operators; arguments have been checked.

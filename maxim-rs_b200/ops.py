@@ -254,6 +254,7 @@ def dense_backward(dy, x, w, pre=None, act="none", slope=0.2, need_dx=True, need
 
 
 def poll():
-    """`mx_dense_poll`: raise if a dense kernel finished so far gave up a wait
-    in its pipeline (its output is then not to be used). Does not wait."""
+    """`mx_dense_poll`: raise if a dense kernel finished so far gave up a wait in
+    its pipeline (its output is then not to be used). Does not wait. Every host
+    thread is told once; until then its dense calls on that device are refused."""
     _native.check(_native.lib().mx_dense_poll(), "dense")

@@ -451,6 +451,53 @@ def test_streams_in_flight_together(ops):
             assert all(torch.equal(a, b) for a, b in zip(r, want[i])), i
 
 
+def test_a_wait_given_up(ops, mx):
+    """A wait that runs out leaves a record: dense calls are refused on every thread
+    until that thread has polled, the norm is not, and afterwards all is as before."""
+    x, w = rand(1, 40, 64), rand(2, 48, 64)
+    want = ops.dense(x, w)
+    ops.poll()
+    lib, stream = mx.lib(), torch.cuda.current_stream().cuda_stream
+    assert lib.mx_dense_wait_check(1000001, stream) == mx._native.MX_E_INVALID
+    assert lib.mx_dense_wait_check(2000, stream) == mx._native.MX_OK
+    torch.cuda.synchronize()
+    for _ in range(2):
+        with pytest.raises(mx.MaximError, match="gave up a wait"):
+            ops.dense(x, w)
+    with pytest.raises(mx.MaximError, match="gave up a wait"):
+        ops.dense_backward(rand(3, 40, 48), x, w)
+    ops.layer_norm(x, w[0], w[1])
+    with pytest.raises(mx.MaximError, match="device 0 gave up a wait"):
+        ops.poll()
+    ops.poll()
+    assert torch.equal(ops.dense(x, w), want)
+    # Two threads: the one's poll leaves the record to the other.
+    seen, used, left = [], threading.Event(), threading.Event()
+
+    def other():
+        ops.dense(x, w)
+        used.set()
+        left.wait(20)
+        for call in (lambda: ops.dense(x, w), ops.poll, ops.poll, lambda: ops.dense(x, w)):
+            try:
+                call()
+                seen.append("taken")
+            except mx.MaximError:
+                seen.append("refused")
+
+    t = threading.Thread(target=other)
+    t.start()
+    assert used.wait(20)
+    assert lib.mx_dense_wait_check(2000, stream) == mx._native.MX_OK
+    torch.cuda.synchronize()
+    with pytest.raises(mx.MaximError):
+        ops.poll()
+    left.set()
+    t.join()
+    assert seen == ["refused", "refused", "taken", "taken"]
+    assert torch.equal(ops.dense(x, w), want)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_calls_read_what_the_call_before_wrote(ops, dtype):
     """Weights that the call just before made (its blocks may still be leaving) serve
