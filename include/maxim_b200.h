@@ -413,7 +413,8 @@ int mx_layer_norm_backward(const mx_layer_norm_backward_args* a, void* stream);
  * form, leaky ReLU with `slope`, the logistic sigmoid. fp32 products are
  * 3xTF32 splits (about 21 significant bits a product, summed in fp32); an
  * infinite fp32 operand gives NaN where it is used. One or two rows (up to
- * eight where w is small) run as plain fp32 sums. y may be the residual itself (same stride). */
+ * eight where w is small) run as plain fp32 sums, in which infinities stay
+ * what they are. y may be the residual itself (same stride). */
 typedef struct mx_dense_args {
   const void* x;
   const void* w;

@@ -454,9 +454,10 @@ __device__ __forceinline__ void dense_tile(const DenseMm& p, int t, int& tm, int
 
 __device__ __forceinline__ float dense_residual(float v) {
   // lo = v - trunc(v), rounded to TF32 (half a TF32 ulp added; the tensor core
-  // drops the low bits itself).
+  // drops the low bits itself). An infinite v leaves a NaN, whose bits may be all
+  // ones: the addition must not carry it past the sign.
   const float hi = __uint_as_float(__float_as_uint(v) & 0xFFFFE000u);
-  return __uint_as_float(__float_as_uint(__fsub_rn(v, hi)) + 0x1000u);
+  return __int_as_float(min(__float_as_int(__fsub_rn(v, hi)), 0x7FFFEFFF) + 0x1000);
 }
 
 // The epilogue of a warp's 32 rows x 32 columns of sums, a row in each lane:

@@ -346,6 +346,29 @@ def test_dense_hard_values(ops):
     assert torch.isinf(ops.dense(big, torch.ones(8, 64, dtype=F16, device="cuda"))).all()
 
 
+@pytest.mark.parametrize("m", [9, 40, 300])
+@pytest.mark.parametrize("other", [1.0, 1.1, -0.3, 2.0 ** -20])  # exact in TF32, and with low bits
+def test_infinite_operands_in_fp32(ops, m, other):
+    """From the tensor cores an infinite fp32 operand gives NaN wherever it is used, whatever it
+    meets; one or two rows give what IEEE does."""
+    for inf in (float("inf"), -float("inf")):
+        x, w = torch.full((m, 64), other, device="cuda"), torch.full((48, 64), other, device="cuda")
+        x[1, 5] = inf
+        w[7, 9] = inf
+        hit = torch.zeros(m, 48, dtype=torch.bool, device="cuda")
+        hit[1], hit[:, 7] = True, True
+        assert torch.equal(torch.isnan(ops.dense(x, w)), hit)
+        few = ops.dense(x[:2], w)
+        assert torch.isinf(few[1]).all() and torch.isinf(few[:, 7]).all()
+        dy = torch.full((m, 48), other, device="cuda")
+        dy[3, 2] = inf
+        dx, dw, db = ops.dense_backward(dy, x, w)
+        assert torch.isnan(dx[3]).all() and torch.isnan(dx[:, 9]).all()
+        assert torch.isfinite(dx[[0, 2, 4]][:, :9]).all()
+        assert torch.isnan(dw[2]).all() and torch.isnan(dw[:, 5]).all() and torch.isfinite(dw[3:, 6:]).all()
+        assert torch.isinf(db[2]) and torch.isfinite(db[[0, 1, 3]]).all()
+
+
 def test_activation_ends(ops):
     """Pre-activations of +-inf and +-1e30 through the activations and their gradients."""
     inf = float("inf")
