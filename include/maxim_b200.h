@@ -347,8 +347,8 @@ int mx_channel_mean_noalloc(const float* x, int64_t npix, int32_t c, int64_t pix
  *     held in fp32, and a result is rounded once, as it is stored;
  *   - `stream` is a cudaStream_t (null: the legacy default stream); calls are
  *     asynchronous on it, allocate nothing (but for 256 bytes of page-locked
- *     host memory at a process's first call, which must come before any
- *     stream capture), and run on the calling thread's current device, which
+ *     host memory at a process's first call), may be captured into a graph, the
+ *     first one too, and run on the calling thread's current device, which
  *     must be able to read the pointers;
  *   - `workspace` is device memory, 16-byte aligned, of at least the bytes
  *     that the _workspace query of the same arguments gives (its pointers

@@ -72,6 +72,14 @@ struct Status {
   WaitRecords records;
   explicit Status(int* w) : words(w), records(w) {}
 };
+// While it lives, this thread may make calls that a stream capture under way
+// (torch's are of the global mode) would refuse and be spoilt by. What is done
+// under it - an allocation kept for good - is no part of any capture.
+struct OutsideCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  OutsideCapture() { MX_CUDA(cudaThreadExchangeStreamCaptureMode(&mode)); }
+  ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
 Status& status() {
   static std::mutex mu;
   static Status* made = nullptr;  // for the life of the process: kernels write it
@@ -79,6 +87,7 @@ Status& status() {
   if (!made) {
     void* p = nullptr;
     constexpr size_t bytes = WaitRecords::kDevices * sizeof(int);
+    OutsideCapture outside;
     MX_CUDA(cudaHostAlloc(&p, bytes, cudaHostAllocPortable | cudaHostAllocMapped));
     std::memset(p, 0, bytes);
     made = new Status(static_cast<int*>(p));
