@@ -414,7 +414,10 @@ int mx_layer_norm_backward(const mx_layer_norm_backward_args* a, void* stream);
  * 3xTF32 splits (about 21 significant bits a product, summed in fp32); an
  * infinite fp32 operand gives NaN where it is used. One or two rows (up to
  * eight where w is small) run as plain fp32 sums, in which infinities stay
- * what they are. y may be the residual itself (same stride). */
+ * what they are. The tensor core cuts its running sums where fp32 would round
+ * them; they are added up in fp32 registers every 64 to 256 of K (fp32) or 4096
+ * (16 bits), so that a sum of one sign comes out low by less than 5e-6 or 3e-5
+ * of itself, however long. y may be the residual itself (same stride). */
 typedef struct mx_dense_args {
   const void* x;
   const void* w;

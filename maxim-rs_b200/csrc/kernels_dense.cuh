@@ -386,11 +386,13 @@ __global__ void __launch_bounds__(256) dense_align_kernel(const __grid_constant_
 //                warps write lo = x - hi to a ring beside it)
 // Two accumulator sets let the epilogue of one tile overlap the products of
 // the next. In fp32 the cross terms hi*lo + lo*hi have a region of their own in
-// a set where TMEM has room for it, and the epilogue takes a set every CHUNK
-// k-blocks and adds it up in registers: the tensor core truncates its accumulator at each MMA,
-// which over a few hundred of them costs more than the products' own rounding
-// (the weights' gradient over 71,680 rows was off by 2.8e-6 of its size with
-// 1,900 rows to a set, by 6.9e-7 with 256).
+// a set where TMEM has room for it. The epilogue takes a set every CHUNK k-blocks
+// and adds it up in registers: the tensor core truncates its accumulator at each
+// MMA, about 1e-7 of a sum of one sign. In fp32 a few hundred of them cost more
+// than the products' own rounding (the weights' gradient over 71,680 rows was off
+// by 2.8e-6 of its size with 1,900 rows to a set, by 6.9e-7 with 256); in 16 bits
+// a few thousand do (131,072 positive rows in one set: 7.8e-4 low, against fp16's
+// rounding of 4.9e-4), and 256 of them lose 2.4e-5.
 // Every wait is bounded in time; one that runs out records a code in the
 // status word and raises the abort flag of both CTAs, on which the other roles
 // stop. The kernel then lets its MMAs end and its copies land, by waits that the
@@ -423,8 +425,9 @@ struct DenseCfg {
   static constexpr int REGIONS = F32 && BN <= 128 ? 2 : 1;  // of an accumulator set: hi*hi and the cross terms, or one
   static constexpr int SET_COLS = REGIONS * BN;
   static constexpr int TMEM_COLS = 2 * SET_COLS;
-  // k-blocks a set accumulates: 32 updates of hi*hi, or 24 of everything.
-  static constexpr int CHUNK = !F32 ? 1 << 30 : (REGIONS == 2 ? 8 : 2);
+  // k-blocks a set accumulates: in fp32 32 updates of hi*hi, or 24 of everything;
+  // in 16 bits 256 updates, 4096 of K.
+  static constexpr int CHUNK = !F32 ? 64 : (REGIONS == 2 ? 8 : 2);
   static constexpr int EPI_WARP0 = 4, EPI_WARPS = BN >= 128 ? 16 : 8;
   static constexpr int EPI_COLS = BN / (EPI_WARPS / 4);  // columns of a tile per epilogue warp
   static constexpr int SPLIT_WARP0 = EPI_WARP0 + EPI_WARPS, SPLIT_WARPS = F32 ? 4 : 0;
@@ -571,11 +574,16 @@ struct DenseOut {
   }
 };
 
-template <class T, bool A_MN, bool B_MN, int BN, int G>
+// CHUNKED: a split may take more than CHUNK k-blocks, so a tile's sums pass
+// through registers (fp32 always, 16 bits past K = 4096. An instance of its own:
+// with both epilogues in one kernel the short products lose 1 to 7%, 71680 x 128
+// -> 256 bf16 with GELU and pre 23.9 to 25.5 us).
+template <class T, bool A_MN, bool B_MN, int BN, int G, bool CHUNKED>
 __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
     dense_mm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmPre, DenseMm p) {
   using C = DenseCfg<T, BN, G>;
+  static_assert(CHUNKED || !C::F32, "fp32 sums always pass through registers");
   using namespace sm100;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -824,7 +832,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
         }
         ++tc;
       };
-      if constexpr (C::F32) {
+      if constexpr (CHUNKED) {
         constexpr int COLS = C::EPI_COLS;
         float sum[COLS];
 #pragma unroll
@@ -852,6 +860,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
 #pragma unroll
         for (int c = 0; c < COLS; c += 32) out.finish(sum + c, split, row0, col0 + c);
       } else {
+        // One set: 32 columns at a time.
         ok = take();
         if (!ok) break;
         const uint32_t d = tmem + (uint32_t(q * 32) << 16) + (tc & 1) * C::SET_COLS + part * C::EPI_COLS;

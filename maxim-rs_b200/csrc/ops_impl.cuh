@@ -331,13 +331,15 @@ CUtensorMap result_map(void* p, int64_t stride, int64_t rows, int64_t cols, int6
   return m;
 }
 
-template <class T, bool A_MN, bool B_MN, int BN, int G>
+template <class T, bool A_MN, bool B_MN, int BN, int G, bool CHUNKED = true>
 void launch_mm(const Operand& a, const Operand& b, const DenseMm& p, int64_t k, const OpsDevice& d, cudaStream_t s) {
   using C = DenseCfg<T, BN, G>;
+  if constexpr (sizeof(T) == 2 && CHUNKED)
+    if (p.kb_split <= C::CHUNK) return launch_mm<T, A_MN, B_MN, BN, G, false>(a, b, p, k, d, s);
   constexpr int kMaxDevices = 64;
   static std::mutex mu;
   static bool opted[kMaxDevices] = {};
-  auto* kernel = dense_mm_kernel<T, A_MN, B_MN, BN, G>;
+  auto* kernel = dense_mm_kernel<T, A_MN, B_MN, BN, G, CHUNKED>;
   {
     int dev = 0;
     MX_CUDA(cudaGetDevice(&dev));
