@@ -7,9 +7,14 @@ most 256 updates in 16 bits, 32 in fp32, each cutting the sum so far by less tha
 2^-20, and both low halves' rounding, 2^-21 each), and every output its own
 rounding. Of one set over 131,072 of K the loss was 7.8e-4."""
 import importlib
+import os
+import sys
 
 import pytest
 import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from test_gpu_ops import DENSE_MKN  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +75,16 @@ def test_products_of_one_sign(ops, mkn, dtype):
     y = ops.dense(x, w)
     ops.poll()
     check(y, sums(x.t(), w.t()))
+
+
+@pytest.mark.parametrize("mkn", DENSE_MKN)
+def test_fp32_split_at_every_size(ops, mkn):
+    """Each of the three products of fp32 operands, where a low half left out or a set that took too much
+    would show (tests/test_fp32_bound.py: what fails this bound)."""
+    m, k, n = mkn
+    x, w, dy = positive(5, m, k, F32), positive(6, n, k, F32), positive(7, m, n, F32)
+    check(ops.dense(x, w), sums(x.t(), w.t()))
+    dx, dw, _ = ops.dense_backward(dy, x, w, need_db=False)
+    check(dx, sums(dy.t(), w))
+    check(dw, sums(dy, x))
+    ops.poll()
