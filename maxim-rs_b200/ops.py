@@ -9,7 +9,9 @@ the library's kernels on the current stream of the tensors' device. Calls
 return without waiting. Tensors are fp32, bf16 or fp16; leading dimensions are
 rows, the last is the row. A tensor whose rows lie apart (a channel range of a
 wider one) is taken as it is; one that is no matrix of contiguous rows (a
-transpose, an expanded gradient) is copied first.
+transpose, an expanded gradient) is copied first. Host threads may call at
+once. layer_norm and dense are known to autograd; the backward calls are there
+for programs that chain them by hand.
 """
 import ctypes
 import struct
@@ -156,10 +158,55 @@ def _launch(entry, layout, values, device, ws_at=None):
     _native.check(getattr(lib, entry)(layout.pack(*values), stream))
 
 
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, scale, bias, eps):
+        y, mean, rstd = layer_norm(x, scale, bias, eps, stats=True)
+        ctx.save_for_backward(x, scale, mean, rstd)
+        ctx.bias_shape = bias.shape
+        ctx.mark_non_differentiable(mean, rstd)
+        return y, mean, rstd
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, _mean, _rstd):
+        need_x, need_scale, need_bias, _ = ctx.needs_input_grad
+        dx, dscale, dbias = layer_norm_backward(dy, *ctx.saved_tensors, need_dx=need_x,
+                                                need_params=need_scale or need_bias)
+        return dx, dscale if need_scale else None, dbias.view(ctx.bias_shape) if need_bias else None, None
+
+
+class _Dense(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, act, slope, save_pre):
+        keep = save_pre or act != "none"
+        y, pre = dense(x, w, bias, act, slope, residual, True) if keep else (dense(x, w, bias, act, slope, residual), None)
+        ctx.save_for_backward(x, w, None if act == "none" else pre)
+        ctx.act, ctx.slope = act, slope
+        ctx.bias_shape = None if bias is None else bias.shape
+        if keep:
+            ctx.mark_non_differentiable(pre)
+        return y, pre
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, _pre):
+        x, w, pre = ctx.saved_tensors
+        need_x, need_w, need_bias, need_residual = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if need_x or need_w or need_bias:
+            dx, dw, db = dense_backward(dy, x, w, pre, ctx.act, ctx.slope, need_x, need_w, need_bias)
+        return dx, dw, db.view(ctx.bias_shape) if need_bias else None, dy if need_residual else None, None, None, None
+
+
 def layer_norm(x, scale, bias, eps=1e-6, stats=False):
     """(x - mean) * rstd * scale + bias over the last dimension. With `stats`
     also the fp32 mean and rstd of every row, which the backward pass takes:
-    (y, mean, rstd). scale and bias are of x's type or fp32."""
+    (y, mean, rstd). scale and bias are of x's type or fp32. Autograd knows of y
+    where an input requires a gradient (mean and rstd carry none)."""
+    if (x.requires_grad or scale.requires_grad or bias.requires_grad) and torch.is_grad_enabled():
+        y, mean, rstd = _LayerNorm.apply(x, scale, bias, eps)
+        return (y, mean, rstd) if stats else y
     device, code = _where(x, scale, bias), _dtype(x)
     xp, rows, c, xs, x = _rows(x, "x")
     pt = _param_dtype(scale, x.dtype)
@@ -205,7 +252,12 @@ def dense(x, w, bias=None, act="none", slope=0.2, residual=None, save_pre=False)
     """act(x @ w.T + bias) + residual: x [..., k], w [n, k], bias [n], residual
     [..., n]. act is one of "none", "gelu" (the erf form), "lrelu" (leaky, with
     `slope`), "sigmoid". With `save_pre` also x @ w.T + bias, which the backward
-    pass of an activation takes: (y, pre)."""
+    pass of an activation takes: (y, pre). Autograd knows of y where an input
+    requires a gradient (pre carries none)."""
+    if ((x.requires_grad or w.requires_grad or bias is not None and bias.requires_grad or
+         residual is not None and residual.requires_grad) and torch.is_grad_enabled()):
+        y, pre = _Dense.apply(x, w, bias, residual, act, slope, save_pre)
+        return (y, pre) if save_pre else y
     device, code = _where(x, w, bias, residual), _dtype(x, w, bias, residual)
     xp, m, k, xs, x = _rows(x, "x")
     if w.dim() != 2:
