@@ -17,9 +17,6 @@ namespace {
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
-template <class T>
-constexpr int kDtype = sizeof(T) == 4 ? MX_DT_F32 : (std::is_same<T, __half>::value ? MX_DT_F16 : MX_DT_BF16);
-
 // Whether every row of a matrix starts on a 16-byte boundary.
 template <class T>
 bool aligned(const void* p, int64_t stride) {
@@ -77,8 +74,11 @@ bool with_norm_shape(int c, F&& f) {
   MX_SHAPE(16, N8)
   MX_SHAPE(32, N8)
   MX_SHAPE(32, N16)
-  if constexpr (!BACKWARD && V > 1) MX_SHAPE(64, N16)
-  MX_SHAPE(128, N8)
+  if constexpr (!BACKWARD && V > 1) {
+    MX_SHAPE(64, N16)  // as many vectors as the next
+  } else {
+    MX_SHAPE(128, N8)
+  }
   MX_SHAPE(128, N16)
   MX_SHAPE(256, N16)
   MX_SHAPE(512, N16)
