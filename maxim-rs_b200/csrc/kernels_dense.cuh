@@ -258,12 +258,14 @@ __global__ void __launch_bounds__(256)
 // d = dy act'(pre) and the partial column sums of d (over fp32 values, before
 // d is rounded to the operands' type for the two products). A block takes
 // lx V columns (lx = 32, or fewer lanes where the matrix is narrow) of a range of
-// rows, 256 / lx rows at a time. With act none, or d null, nothing is written but
-// the sums. GELU's derivative is about 17 instructions an element, which in 16
-// bits is as long as the memory's time. With an activation, what is read here
-// leaves the L2 first, so that more of d is still there for the products
-// (gradient of 71680 x 128 -> 256 fp32: 105 us to 101).
-template <class T, int V>
+// rows, 256 / lx rows at a time. Without STORE (no product wants d, or act is none and
+// d is dy) nothing is written but the sums. GELU's derivative is about 17 instructions an element, which in 16
+// bits is as long as the memory's time. Where d is stored, what is read here leaves
+// the L2 first, so that more of d is still there for the products (gradients from 1000
+// x 256 -> 1024 to 8192 x 4096 -> 4096 in each type: 0.97 to 1.00 of the time with
+// ordinary loads, 1.01 for the smallest). The sums alone take 1.02 of their time with
+// such loads, and have an instance without: a choice inside the loop costs as much.
+template <class T, int V, bool STORE>
 __global__ void __launch_bounds__(256, 3)
     dense_grad_kernel(const T* dy, int64_t dy_stride, const T* pre, int64_t pre_stride, T* d, int64_t d_stride,
                       float* part, T* db, int64_t m, int n, int lx_log2, int act, float slope) {
@@ -285,11 +287,12 @@ __global__ void __launch_bounds__(256, 3)
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
         const int64_t r = r0 + i * step;
-        if (act == MX_ACT_NONE) {
-          dr[i] = r < m ? raw_load<T, V>(dy + r * dy_stride + col) : raw_zero<T, V>();
-        } else {
+        if constexpr (STORE) {
           dr[i] = r < m ? raw_load_streaming<T, V>(dy + r * dy_stride + col) : raw_zero<T, V>();
           pr[i] = r < m ? raw_load_streaming<T, V>(pre + r * pre_stride + col) : raw_zero<T, V>();
+        } else {
+          dr[i] = r < m ? raw_load<T, V>(dy + r * dy_stride + col) : raw_zero<T, V>();
+          if (act != MX_ACT_NONE) pr[i] = r < m ? raw_load<T, V>(pre + r * pre_stride + col) : raw_zero<T, V>();
         }
       }
 #pragma unroll
@@ -297,14 +300,14 @@ __global__ void __launch_bounds__(256, 3)
         const int64_t r = r0 + i * step;
         float v[V];
         raw_unpack<T, V>(dr[i], v);
-        if (act != MX_ACT_NONE) {
+        if (STORE || act != MX_ACT_NONE) {
           float q[V];
           raw_unpack<T, V>(pr[i], q);
           apply_act_grad<V>(act, v, q, slope);
-          if (d && r < m) raw_store<T, V>(d + r * d_stride + col, raw_pack<T, V>(v));
+          if (STORE && r < m) raw_store<T, V>(d + r * d_stride + col, raw_pack<T, V>(v));
         }
 #pragma unroll
-        for (int k = 0; k < V; ++k) a[k] += v[k];
+        for (int k = 0; k < V; ++k) a[k] = __fadd_rn(a[k], v[k]);  // not contracted: the same sums with STORE and without
       }
     }
   }

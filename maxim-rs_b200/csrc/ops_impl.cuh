@@ -584,17 +584,23 @@ void dense_backward(const mx_dense_backward_args& a, const OpsDevice& dev, cudaS
   Carver c{static_cast<uint8_t*>(a.workspace)};
   DenseBackward<T> b(c, a, dev);
   if (b.chunks) {
-    auto go = [&](auto v) {
-      constexpr int V = decltype(v)::value;
-      launch_clusters(dense_grad_kernel<T, V>, dim3(unsigned(b.cols), unsigned(b.chunks)), dim3(256), 0,
+    auto go = [&](auto v, auto store) {
+      launch_clusters(dense_grad_kernel<T, decltype(v)::value, decltype(store)::value>,
+                      dim3(unsigned(b.cols), unsigned(b.chunks)), dim3(256), 0,
                       b.cluster ? dim3(1, unsigned(b.chunks)) : dim3(1), s, static_cast<const T*>(a.dy), a.dy_stride,
                       static_cast<const T*>(a.pre), a.pre_stride, b.d, b.d_stride, b.db_part,
                       b.cluster ? static_cast<T*>(a.db) : nullptr, a.m, int(a.n), b.lx_log2, int(a.act), a.slope);
     };
+    auto by_store = [&](auto v) {
+      if (b.d)
+        go(v, std::true_type());
+      else
+        go(v, std::false_type());
+    };
     if (b.vec)
-      go(std::integral_constant<int, kVec<T>>());
+      by_store(std::integral_constant<int, kVec<T>>());
     else
-      go(std::integral_constant<int, 1>());
+      by_store(std::integral_constant<int, 1>());
     if (b.db_part) join_columns<T>(b.db_part, b.chunks, a.n, a.n, a.db, nullptr, false, s);
   }
   if (!b.products) return;
