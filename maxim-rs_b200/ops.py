@@ -305,6 +305,12 @@ def dense_backward(dy, x, w, pre=None, act="none", slope=0.2, need_dx=True, need
     return dx, dw, db
 
 
+def release_workspaces():
+    """Give the workspaces that the calling thread's calls have kept (up to 32 MB a
+    stream) back to torch's allocator. A thread's go with the thread by themselves."""
+    _kept.by_stream.clear()
+
+
 def poll():
     """`mx_dense_poll`: raise if a dense kernel finished so far gave up a wait in
     its pipeline (its output is then not to be used). Does not wait. Every host

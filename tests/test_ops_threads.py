@@ -1,8 +1,10 @@
 """The operators' torch binding called from several host threads, with a stand-in
 for the library: no call may be given device memory that another may still use."""
+import gc
 import importlib
 import struct
 import threading
+import weakref
 
 import pytest
 
@@ -81,3 +83,33 @@ def test_a_thread_keeps_its_workspace(ops, monkeypatch):
     for _ in range(3):
         ops._launch("mx_op", layout, [1, 2, 0, 0], 0, 2)
     assert len(set(lib.taken)) == 1
+
+
+def test_kept_workspaces_can_be_released(ops, monkeypatch):
+    """By the thread that keeps them; another thread's go with it."""
+    layout = struct.Struct("<2Q2q")
+    monkeypatch.setattr(ops._native, "lib", lambda: Library(layout, 2, 1))
+    made = []
+    empty = ops.torch.empty
+
+    def recording(*a, **kw):
+        t = empty(*a, **kw)
+        made.append(weakref.ref(t))
+        return t
+
+    monkeypatch.setattr(ops.torch, "empty", recording)
+
+    def call():
+        ops._launch("mx_op", layout, [1, 2, 0, 0], 0, 2)
+
+    call()
+    t = threading.Thread(target=call)
+    t.start()
+    t.join()
+    gc.collect()
+    assert [r() is not None for r in made] == [True, False]
+    ops.release_workspaces()
+    gc.collect()
+    assert made[0]() is None
+    call()
+    assert len(made) == 3
