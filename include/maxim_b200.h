@@ -412,11 +412,12 @@ int mx_layer_norm_backward(const mx_layer_norm_backward_args* a, void* stream);
  * convolution's [c_out][c_in]), y [m][n]. act is MX_ACT_*: GELU in its erf
  * form, leaky ReLU with `slope`, the logistic sigmoid. fp32 products are
  * 3xTF32 splits (about 21 significant bits a product, summed in fp32); an
- * infinite fp32 operand gives NaN where it is used. One or two rows (up to
+ * infinite fp32 operand gives NaN where it is used, and one below 2^-118 keeps
+ * fewer bits the smaller it is. One or two rows (up to
  * eight where w is small) run as plain fp32 sums, in which infinities stay
  * what they are. The tensor core cuts its running sums where fp32 would round
  * them; they are added up in fp32 registers every 64 to 256 of K (fp32) or 4096
- * (16 bits), so that a sum of one sign comes out low by less than 5e-6 or 3e-5
+ * (16 bits), so that a sum of one sign comes out low by less than 6e-6 or 3e-5
  * of itself, however long. y may be the residual itself (same stride). */
 typedef struct mx_dense_args {
   const void* x;
