@@ -379,7 +379,8 @@ __global__ void __launch_bounds__(256) dense_align_kernel(const __grid_constant_
 // (8192 x 4096 -> 8192 bf16: 418 us with one CTA a tile, 363 with two).
 // One CTA per SM, persistent over the tiles. Warp roles:
 //   warp 0       TMA producer: 128 bytes of K (64 or 32 elements) a stage
-//   warp 1       MMA issuer (one lane, of the pair's leader)
+//   warp 1       MMA issuer (one lane, of the pair's leader; the peer's passes on
+//                that its lo tiles are written)
 //   warp 2       TMEM owner
 //   warps 4-19   epilogue: TMEM -> registers -> bias, activation, residual ->
 //   (or 4-11)    shared memory -> TMA store; four (two) warps per TMEM lane
@@ -421,8 +422,9 @@ struct DenseCfg {
   static constexpr int B_BYTES = BROWS * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   // fp32: the lo halves have a shorter ring of their own, so that more of the
-  // shared memory holds loads in flight.
-  static constexpr int LO_STAGES = F32 ? 2 : 0;
+  // shared memory holds loads in flight. A pair's is one longer, for the time that
+  // word of the peer's takes (4096^3 658 to 621 us, 71680 x 128 -> 256 40.8 to 39.2).
+  static constexpr int LO_STAGES = F32 ? (G == 2 ? 3 : 2) : 0;
   static constexpr int FIT = 192 * 1024 / STAGE_BYTES - LO_STAGES;
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
   static constexpr int REGIONS = F32 && BN <= 128 ? 2 : 1;  // of an accumulator set: hi*hi and the cross terms, or one
@@ -443,7 +445,7 @@ struct DenseCfg {
   static_assert(!SPLIT_REGS || (THREADS == 768 && REGS_CONTROL + 4 * REGS_EPI + REGS_SPLIT <= 480), "register split");
   static constexpr int STAGING_BYTES = EPI_WARPS * 2048;  // 32 rows x 64 bytes each
   static constexpr int SMEM_BYTES =
-      1024 + (STAGES + LO_STAGES) * STAGE_BYTES + STAGING_BYTES + 8 * (2 * STAGES + 2 * LO_STAGES + 5) + 16;
+      1024 + (STAGES + LO_STAGES) * STAGE_BYTES + STAGING_BYTES + 8 * (2 * STAGES + 3 * LO_STAGES + 5) + 16;
   static_assert(SMEM_BYTES <= 232448 - 64, "shared memory per CTA");
   static_assert(TMEM_COLS <= 512, "TMEM columns");
 };
@@ -598,7 +600,8 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
   uint64_t* lo_empty = lo_ready + C::LO_STAGES;
   uint64_t* acc_full = lo_empty + C::LO_STAGES;
   uint64_t* acc_empty = acc_full + 2;
-  uint64_t* drained = acc_empty + 2;
+  uint64_t* peer_lo_ready = acc_empty + 2;  // in a pair's leader: the peer's lo_ready, passed on
+  uint64_t* drained = peer_lo_ready + C::LO_STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   __shared__ int abort_flag;
   __shared__ uint32_t issued;  // stages that this CTA's producer has loaded
@@ -619,7 +622,8 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < C::LO_STAGES; ++s) {
-      mbar_init(&lo_ready[s], G * C::SPLIT_WARPS);
+      mbar_init(&lo_ready[s], C::SPLIT_WARPS);
+      mbar_init(&peer_lo_ready[s], 1);
       mbar_init(&lo_empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -763,7 +767,11 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
               d = tmem + acc * C::SET_COLS;
               left = min(C::CHUNK, k1 - kb);
             }
-            ok = __all_sync(0xFFFFFFFFu, C::F32 ? wait_pair(&lo_ready[l], lph) : wait_pair(&full[s], ph));
+            if constexpr (C::F32)
+              ok = wait(&lo_ready[l], lph) && (G == 1 || wait_order(&peer_lo_ready[l], lph));
+            else
+              ok = wait_pair(&full[s], ph);
+            ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) {
               if (lane == 0) fail(kDenseErrMmaStage);
               break;
@@ -802,6 +810,25 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
         if (elect_one()) commit(drained);
         __syncwarp();
         if (!__all_sync(0xFFFFFFFFu, mbar_wait(drained, 0, nullptr)) && lane == 0) fail(kDenseErrDrain);
+      } else if (C::F32 && lane == 0) {
+        // The peer's lo tiles, as its split warps write them, for the leader's MMAs.
+        // Here, so that the fence does not hold those warps up.
+        uint32_t l = 0, lph = 0;
+        bool ok = true;
+        for (int w = first; w < items && ok; w += step) {
+          int k0, k1;
+          kb_range(w / tiles, k0, k1);
+          for (int kb = k0; kb < k1; ++kb) {
+            ok = wait(&lo_ready[l], lph);
+            if (!ok) {
+              fail(kDenseErrMmaStage);
+              break;
+            }
+            fence_async_release_cluster();
+            mbar_arrive_cluster(map_rank(&peer_lo_ready[l], 0));
+            if (++l == C::LO_STAGES) l = 0, lph ^= 1;
+          }
+        }
       }
     }
   } else if (warp < C::SPLIT_WARP0) {
@@ -912,14 +939,7 @@ __global__ void __launch_bounds__(DenseCfg<T, BN, G>::THREADS, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (G == 2) {
-            fence_async_release_cluster();
-            mbar_arrive_cluster(map_rank(&lo_ready[l], 0));
-          } else {
-            mbar_arrive(&lo_ready[l]);
-          }
-        }
+        if (lane == 0) mbar_arrive(&lo_ready[l]);
         if (++s == C::STAGES) s = 0, ph ^= 1;
         if (++l == C::LO_STAGES) l = 0, lph ^= 1;
       }
