@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(_HERE, "libmaxim_b200.so")
 
 MX_OK = 0
 MX_E_INVALID = -1
+MX_E_DEVICE = -6
 OP_NAMES = ["copy", "add", "mul", "gate_apply", "gelu", "lrelu", "sigmoid", "chan_ln", "chan_mean", "chan_scale",
             "conv1x1", "conv3x3", "conv4x4s2", "convt2x2", "gate_mm", "block_perm", "resize", "down_s"]
 

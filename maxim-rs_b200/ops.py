@@ -195,7 +195,14 @@ class _Dense(torch.autograd.Function):
         need_x, need_w, need_bias, need_residual = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if need_x or need_w or need_bias:
-            dx, dw, db = dense_backward(dy, x, w, pre, ctx.act, ctx.slope, need_x, need_w, need_bias)
+            try:
+                dx, dw, db = dense_backward(dy, x, w, pre, ctx.act, ctx.slope, need_x, need_w, need_bias)
+            except _native.MaximError as e:
+                # Nobody can poll on autograd's own thread: its records are told by this error.
+                if e.code == _native.MX_E_DEVICE:
+                    while _native.lib().mx_dense_poll() == _native.MX_E_DEVICE:
+                        pass
+                raise
         return dx, dw, db.view(ctx.bias_shape) if need_bias else None, dy if need_residual else None, None, None, None
 
 

@@ -106,6 +106,25 @@ def test_second_gradients_are_refused(ops):
         dx.sum().backward()
 
 
+def test_a_wait_given_up_is_told_by_the_backward_pass(ops, mx):
+    """Autograd runs it on a thread of its own, on which nobody can poll: the error is raised once."""
+    x, w = rand(1, 40, 48).requires_grad_(), rand(2, 80, 48).requires_grad_()
+    ops.dense(x, w).sum().backward()  # that thread has made a call
+    y = ops.dense(x, w).sum()
+    assert mx.lib().mx_dense_wait_check(2000, torch.cuda.current_stream().cuda_stream) == mx._native.MX_OK
+    torch.cuda.synchronize()
+    with pytest.raises(mx.MaximError, match="gave up a wait"):
+        y.backward()
+    with pytest.raises(mx.MaximError, match="gave up a wait"):
+        ops.dense(x, w)
+    with pytest.raises(mx.MaximError, match="gave up a wait"):
+        ops.poll()
+    x.grad = None
+    ops.dense(x, w).sum().backward()
+    assert torch.allclose(x.grad, w.detach().sum(0).expand(40, 48), rtol=1e-5, atol=1e-4)
+    ops.poll()
+
+
 def test_threads_train_on_one_stream(ops):
     """Forward calls on this thread while autograd's own thread runs another's backward pass."""
     x, w = rand(1, 700, 512, dtype=torch.bfloat16), rand(2, 1000, 512, dtype=torch.bfloat16, scale=0.03)
