@@ -79,10 +79,14 @@ __device__ __forceinline__ void row_sum(float (&s)[K], float (*red)[32 * K], int
 template <int L>
 constexpr int kNormThreads = L <= 32 ? 256 : L;
 // Blocks an SM is asked to hold (0: the compiler's own choice of registers).
-// Asking for one lets a row's block have more of them: 20000 x 1000 fp16 backward
-// 40 to 35 us, 32768 x 2048 bf16 forward 51 to 46; the other shapes lose by it.
+// Asking for one lets a row's block have more of them, and fewer blocks share the
+// SM. Time with it over time without, 64 to 128 MB of rows: forward 0.92 to 0.99 for 128
+// lanes or fewer, 0.83 to 0.97 for fp32 rows of 256, 0.86 to 0.96 for 512 (1.05 at fp32 rows of
+// 8192); but 1.05 to 1.12 for 16-bit rows of 256 lanes (2056 to 4096 long, which the
+// compiler gives three blocks of fewer registers by itself). Backward 0.91 to 0.97 for 128
+// and 512 lanes in 16 bits, 0.95 to 1.01 in fp32.
 template <int V, int L, bool BACKWARD>
-constexpr int kNormMinBlocks = BACKWARD ? (L == 128 || L == 512) : (V > 1 && L > 32);
+constexpr int kNormMinBlocks = BACKWARD ? (L == 128 || L == 512) : (V > 1 && L > 32 && !(V == 8 && L == 256));
 // Up to 16 values a thread the parameters and the next row fit in registers too.
 template <int V, int NV>
 constexpr bool kNormHold = V * NV <= 16;
